@@ -394,6 +394,49 @@ int b200moe_ep_return_rows(const void* y_pos_bf16, const int32_t* row_valid, con
                            void* const* back_peers, int world, int64_t cap_rows, int H, int64_t back_rows,
                            b200moe_stream_t stream);
 
+/* ---- training pass of the experts -----------------------------------------------------------------
+ * No counterpart in the reference's inference kernels.  Rows are sorted by expert without padding: expert e owns rows expert_offsets[e] to expert_offsets[e + 1] (int32 [E + 1], on the device) of R = T * K rows, E <= 1024.
+ *
+ * sort_pairs: order of the pairs p = t * K + k of expert_index [T, K] (index_bytes 4 or 8) by (expert, p).  row_of_pair [T, K]
+ * gets a pair's row, -1 where the id lies outside [0, E); pair_of_row [T * K] the pair of a row, -1 behind the last expert. */
+size_t b200moe_sort_workspace_bytes(int64_t pairs, int E);
+int b200moe_sort_pairs(const void* expert_index, int index_bytes, int T, int K, int E, int32_t* expert_offsets,
+                       int32_t* row_of_pair, int32_t* pair_of_row, void* workspace, size_t workspace_bytes,
+                       b200moe_stream_t stream);
+/* rows[row_of_pair[t, k]] = hidden[t]; rows behind the last expert become zero.  dtype F32 or BF16, pitches in elements;
+ * outputs are contiguous. */
+int b200moe_sort_rows(const void* hidden, int dtype, int64_t pitch, int T, int K, int H, int E,
+                      const int32_t* row_of_pair, const int32_t* expert_offsets, void* rows, b200moe_stream_t stream);
+/* out[t] = sum over k of affinities[t, k] rows[row_of_pair[t, k]] in fp32, k ascending, one rounding.  affinities [T, K]
+ * (aff_dtype) or NULL = 1, which makes it the gradient of sort_rows. */
+int b200moe_unsort_rows(const void* rows, int dtype, int64_t pitch, int T, int K, int H, const int32_t* row_of_pair,
+                        const void* affinities, int aff_dtype, void* out, b200moe_stream_t stream);
+/* Its gradients: d_rows[r] = affinities[t, k] d_out[t], zero behind the last expert; d_affinities[t, k] (aff_dtype) =
+ * <d_out[t], rows[r]>, zero for a pair without a row.  Either may be NULL. */
+int b200moe_unsort_rows_backward(const void* d_out, int64_t d_pitch, const void* rows, int64_t pitch, int dtype, int T,
+                                 int K, int H, int E, const int32_t* row_of_pair, const int32_t* expert_offsets,
+                                 const void* affinities, int aff_dtype, void* d_rows, void* d_affinities,
+                                 b200moe_stream_t stream);
+/* Every expert's rows times its matrix, bf16 with fp32 accumulation.  weight: E matrices [D0, D1] with D1 contiguous
+ * (pitches in elements).  contract_last 0: rows [R, D0] -> out [R, D1]; 1: rows [R, D1] -> out [R, D0].  Rows of no expert
+ * come out zero.  D0 and D1 are multiples of 8; rows and matrices start on 16-byte boundaries.  status as for the grouped
+ * contractions (codes 41 to 46). */
+int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch, const void* weight_bf16, int64_t w_pitch,
+                           int64_t w_expert_pitch, int contract_last, const int32_t* expert_offsets, int R, int E, int D0,
+                           int D1, void* out_bf16, int32_t* status, b200moe_stream_t stream);
+/* out[e] [M, N] = sum over the expert's rows r of a[r, :]^T b[r, :]; zero for an expert without rows. */
+int b200moe_expert_weight_grad(const void* a_bf16, int64_t a_pitch, const void* b_bf16, int64_t b_pitch,
+                               const int32_t* expert_offsets, int R, int E, int M, int N, void* out_bf16, int32_t* status,
+                               b200moe_stream_t stream);
+/* m [R, I] = act(gate) * up of gate_up [R, 2 I] (gate first), I a multiple of 8.  codes [R, 2 I] e4m3 and scales
+ * [R, 2, ceil(I / 32)] UE8M0 (both NULL: not kept): v is kept as e4m3(v / s), s the smallest power of two of at least 2^-127
+ * for which no finite value of the 32 columns exceeds 448 s; a value that is not finite is kept as NaN. */
+int b200moe_glu(const void* gate_up_bf16, int64_t pitch, int64_t R, int I, int act_fn, void* m_bf16, uint8_t* codes,
+                uint8_t* scales, b200moe_stream_t stream);
+/* From the kept g and u: d_gate_up [R, 2 I] = (d_m u act'(g), d_m act(g)) and m [R, I] = act(g) u.  Either may be NULL. */
+int b200moe_glu_backward(const void* d_m_bf16, int64_t pitch, const uint8_t* codes, const uint8_t* scales, int64_t R, int I,
+                         int act_fn, void* d_gate_up_bf16, void* m_bf16, b200moe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

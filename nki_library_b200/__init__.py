@@ -12,6 +12,9 @@ Public entry points mirror the reference (paths relative to its root):
 ``moe_block_tkg``      core/moe_block/moe_block_tkg.py:39
 =====================  ==========================================================
 
+and, without a counterpart there, the experts' training pass: ``moe_sort_plan``, ``moe_sort_tokens``,
+``moe_unsort_tokens``, ``expert_linear``, ``moe_glu``, ``moe_expert_mlp``, ``moe_experts_train``.
+
 All of them run hand-written sm_100a CUDA kernels through the C ABI in
 ``include/b200moe.h``; there is no CPU implementation in this package.
 """
@@ -30,6 +33,16 @@ from .core.moe.moe_cte import (  # noqa: F401
     moe_group_tokens,
 )
 from .core.moe.moe_tkg import moe_tkg  # noqa: F401
+from .core.moe.moe_train import (  # noqa: F401
+    SortedTokens,
+    expert_linear,
+    moe_expert_mlp,
+    moe_experts_train,
+    moe_glu,
+    moe_sort_plan,
+    moe_sort_tokens,
+    moe_unsort_tokens,
+)
 from .core.moe_block import moe_block_tkg  # noqa: F401
 from .core.router_topk import router_topk  # noqa: F401
 from .core.subkernels import find_nonzero_indices, indexed_flatten  # noqa: F401

@@ -1,0 +1,75 @@
+"""The experts' part of a training step: sort, gate/up product, gated activation, down product, weighted sum."""
+
+from __future__ import annotations
+
+import torch
+
+from .... import _lib
+from ...utils.common_types import ActFnType
+from .expert_linear import check_rows_and_weight, product, weight_grad
+from .launch import needs_grad, same_device, tile_rows
+from .moe_glu import glu_backward, glu_forward
+from .sort_tokens import moe_sort_tokens, moe_unsort_tokens
+
+
+class _ExpertMLP(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, gate_up_weight, down_weight, expert_offsets, act):
+        m, codes, scales = glu_forward(product(rows, gate_up_weight, expert_offsets), act, True)
+        ctx.save_for_backward(rows if gate_up_weight.requires_grad else None, gate_up_weight, down_weight, expert_offsets,
+                              codes, scales)
+        ctx.act = act
+        return product(m, down_weight, expert_offsets)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out):
+        rows, gate_up_weight, down_weight, offsets, codes, scales = ctx.saved_tensors
+        want_rows, want_gate_up, want_down = ctx.needs_input_grad[:3]
+        d_out = tile_rows(d_out)
+        d_m = product(d_out, down_weight, offsets, transpose=True)
+        d_gate_up, m = glu_backward(d_m, codes, scales, ctx.act, want_m=want_down)
+        d_down = weight_grad(m, d_out, down_weight, offsets) if want_down else None
+        d_rows = product(d_gate_up, gate_up_weight, offsets, transpose=True) if want_rows else None
+        d_gate_up_weight = weight_grad(rows, d_gate_up, gate_up_weight, offsets) if want_gate_up else None
+        return d_rows, d_gate_up_weight, d_down, None, None
+
+
+def moe_expert_mlp(rows: torch.Tensor, gate_up_proj_weight: torch.Tensor, down_proj_weight: torch.Tensor,
+                   expert_offsets: torch.Tensor, activation_function: ActFnType = ActFnType.SiLU) -> torch.Tensor:
+    """The experts' MLP on sorted rows: ``(act(gate) * up) @ down_proj_weight[e]`` with ``[gate, up] = rows @
+    gate_up_proj_weight[e]``; ``rows [R, H]``, weights ``[E, H, 2, I]`` (or ``[E, H, 2 I]``) and ``[E, I, H]``, all bf16.
+
+    The three operators in a row (:func:`expert_linear`, :func:`moe_glu`, :func:`expert_linear`), but what lives until the
+    backward pass is the input rows and the 8-bit checkpoint of gate and up only: the activation in front of the down
+    product is computed again from the checkpoint for the gradient of ``down_proj_weight``.
+    """
+    same_device(rows, gate_up_proj_weight, down_proj_weight, expert_offsets)
+    A = _lib.kernel_assert
+    if gate_up_proj_weight.dim() == 4:
+        gate_up_proj_weight = gate_up_proj_weight.flatten(2)
+    check_rows_and_weight(rows, gate_up_proj_weight, expert_offsets, "gate_up_proj_weight")
+    A(isinstance(activation_function, ActFnType), "activation_function must be an ActFnType")
+    A(down_proj_weight.dim() == 3 and down_proj_weight.dtype == torch.bfloat16 and
+      down_proj_weight.shape[0] == gate_up_proj_weight.shape[0] and
+      2 * down_proj_weight.shape[1] == gate_up_proj_weight.shape[2], "down_proj_weight must be bfloat16 [E, I, H_out]")
+    A(down_proj_weight.shape[1] % 8 == 0 and down_proj_weight.shape[2] % 8 == 0 and down_proj_weight.shape[2] > 0,
+      "both sizes of down_proj_weight's matrices must be multiples of 8")
+    act = activation_function.value
+    if needs_grad(rows, gate_up_proj_weight, down_proj_weight):
+        return _ExpertMLP.apply(rows, gate_up_proj_weight, down_proj_weight, expert_offsets, act)
+    m = glu_forward(product(rows, gate_up_proj_weight, expert_offsets), act, False)[0]
+    return product(m, down_proj_weight, expert_offsets)
+
+
+def moe_experts_train(hidden: torch.Tensor, affinities: torch.Tensor, expert_index: torch.Tensor,
+                      gate_up_proj_weight: torch.Tensor, down_proj_weight: torch.Tensor,
+                      activation_function: ActFnType = ActFnType.SiLU) -> torch.Tensor:
+    """The MoE layer behind its router, differentiable in ``hidden [T, H]``, ``affinities [T, K]`` and both weights:
+    :func:`moe_sort_tokens` -> :func:`moe_expert_mlp` -> :func:`moe_unsort_tokens`.  ``expert_index [T, K]`` may hold ids
+    outside ``[0, E)`` for dropped pairs; a token whose pairs are all dropped comes out zero.
+    """
+    same_device(hidden, affinities, expert_index, gate_up_proj_weight, down_proj_weight)
+    rows, plan = moe_sort_tokens(hidden, expert_index, gate_up_proj_weight.shape[0])
+    out = moe_expert_mlp(rows, gate_up_proj_weight, down_proj_weight, plan.expert_offsets, activation_function)
+    return moe_unsort_tokens(out, affinities, plan)
