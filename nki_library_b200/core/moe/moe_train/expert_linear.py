@@ -38,12 +38,12 @@ def product(rows: torch.Tensor, weight: torch.Tensor, expert_offsets: torch.Tens
         return out
     rows = tile_rows(rows)
     w_pitch = stored.stride(1)
-    status = torch.empty(1, dtype=torch.int32, device=rows.device)
+    status = torch.empty(2, dtype=torch.int32, device=rows.device)
     launch(rows.device, "b200moe_expert_product", rows.data_ptr(), pitch_of(rows), stored.data_ptr(), w_pitch,
            stored.stride(0) if E > 1 else D0 * w_pitch, int(contract_last), expert_offsets.data_ptr(), R, E, D0, D1,
            out.data_ptr(), status.data_ptr())
     if check_status:
-        _lib.kernel_assert(int(status.item()) == 0, f"device-side wait expired in expert_linear (status {int(status.item())})")
+        _lib.kernel_assert(int(status[0].item()) == 0, f"device-side wait expired in expert_linear (status {int(status[0].item())})")
     return out
 
 
@@ -58,7 +58,7 @@ def weight_grad(rows: torch.Tensor, d_out: torch.Tensor, weight: torch.Tensor, e
     else:
         out = torch.empty((E, M, W), dtype=torch.bfloat16, device=weight.device)
         a, b = tile_rows(a), tile_rows(b)
-        status = torch.empty(1, dtype=torch.int32, device=weight.device)
+        status = torch.empty(2, dtype=torch.int32, device=weight.device)
         launch(weight.device, "b200moe_expert_weight_grad", a.data_ptr(), pitch_of(a), b.data_ptr(), pitch_of(b),
                expert_offsets.data_ptr(), rows.shape[0], E, M, W, out.data_ptr(), status.data_ptr())
     return out.transpose(1, 2) if turned else out

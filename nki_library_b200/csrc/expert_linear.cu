@@ -1,23 +1,30 @@
 // Products of sorted token rows with their experts' matrices, and the gradients of those products, in bf16 with fp32
 // accumulation on the sm_100a tensor cores.  Expert e owns rows [offsets[e], offsets[e + 1]) of a row matrix.
 //
-//   product      out[r, n] = sum_k rows[r, k] op(W[e])[k, n]     contraction over either axis of the stored matrix
-//   weight grad  out[e][m, n] = sum over the expert's rows r of a[r, m] b[r, n]
+//   product      out[r, c] = sum_k rows[r, k] op(W[e])[k, c]     contraction over either axis of the stored matrix
+//   weight grad  out[e][m, c] = sum over the expert's rows r of a[r, m] b[r, c]
 //
 // Nothing is transposed in memory: the matrix descriptors of tcgen05 read an operand whose contraction axis is contiguous
 // ("K-major": 64 elements of it are one 128-byte row of a swizzled tile) as well as one whose other axis is ("MN-major": a
 // tile is 64 contraction steps of 64 contiguous outputs).  Forward reads W [K, N] MN-major, the gradient of the rows reads
 // the same W K-major, the gradient of W reads both row matrices MN-major.
 //
-// A tile is 256 x 256 outputs on a CTA pair (cta_group::2): each CTA loads 128 rows of either operand per 64 contraction
-// steps (32 KB), i.e. 64 bytes per SM and tensor-pipe clock, the smallest feed that two accumulators in TMEM allow.
+// Output columns are the M side of every MMA and output rows the N side: a tile is 256 columns x up to 256 rows on a CTA
+// pair (cta_group::2), and an expert's rows are cut into tiles of nearly equal width, any multiple of 32, so that an odd
+// load costs no padding to 256 and a few rows cost a stream of weights and little else.  Each CTA loads 128 of the columns
+// and half of the rows per 64 contraction steps, 64 bytes per SM and tensor-pipe clock for a full tile, the smallest feed
+// that two accumulators in TMEM allow.
 //
-// Warps of a persistent CTA (384 threads):
-//   0, 3   TMA producers of the A and the B operand
-//   1      allocates TMEM; in the even CTA issues the MMAs (M 256, N 256, K 16)
-//   2      weight grad: clears the rows of a contraction's last 16 that belong to the next expert (or hold what a caller
-//          left behind the last one), so that they add nothing, whatever they hold
-//   4..11  epilogue: accumulator lane = output row, two warps per 32 lanes take 128 columns each
+// Warps of a persistent CTA (256 threads, weight grad 384):
+//   0, 3   TMA producers of the column and the row operand
+//   1      allocates TMEM; in the even CTA issues the MMAs (M 256, K 16), in the odd one hands out the pair's tiles
+//   2      weight grad: fetches the rows of a contraction that do not fill a step of 16 into a buffer of their own and
+//          clears those behind them, which belong to the next expert (or hold what a caller left behind the last one), so
+//          that they add nothing, whatever they hold
+//   4..    epilogue: groups of four warps take chunks of 32 output rows in turn.  An accumulator lane is an output column, so
+//          the 32 values a warp holds of a row are 64 contiguous bytes and go straight out.  Turning a chunk around in
+//          shared memory for longer stores costs the tensor pipe operand bandwidth, which the ring's copies and the MMAs
+//          use up (4 x 1024 rows, 4096 x 14336, weight grad: 361 us turned, 353 straight; 32 x 16 rows, 4096 x 4096: 248, 194).
 // Every wait is bounded; on expiry a code goes to `status`, no more work is issued and the kernel tears down.
 #include <cuda.h>
 
@@ -28,38 +35,64 @@ namespace b200moe {
 namespace {
 
 constexpr int kMaxExperts = 1024;
-constexpr int kThreads = 384;
 constexpr int kStages = 6;
 constexpr int kOperand = 128 * 128;  // bytes of one operand's part of a stage: 128 rows of 128 bytes
 constexpr int kStage = 2 * kOperand;
-constexpr int kGroup = 8;  // row tiles that are walked together for every column tile: they share a weight tile in L2
+constexpr int kGroup = 8;    // row tiles that are walked together for every column tile: they share a weight tile in L2
+constexpr int kTail = 4 * 2048;  // weight grad: 16 contraction rows of either operand, two boxes of 64 outputs each
+
+// n / d for 0 <= n < 2^31 without a division: n * m >> 31 + s with m the reciprocal rounded up (1 <= d < 2^30).
+struct Divisor {
+  uint32_t d, m;
+  int s;
+  __device__ __forceinline__ int quotient(int n) const {
+    return d == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), m) >> (s - 1));
+  }
+};
+inline Divisor make_divisor(uint32_t d) {
+  int s = 0;
+  while ((1u << s) < d) ++s;
+  return {d, static_cast<uint32_t>(((uint64_t{1} << (31 + s)) / d) + 1), s};
+}
 
 struct Params {
   const int32_t* offsets;
   int R, E;
-  int m, n;         // weight grad: its matrix; product: n output columns
-  int k;            // product: contraction length
-  int m_tiles, n_tiles;  // product: m_tiles unused
+  int rows, cols;  // weight grad: the size of its matrices; product: output columns
+  int k;           // product: contraction length
+  int row_tiles, col_tiles;  // product: row_tiles unused
+  Divisor per_matrix, per_group;  // tiles of a matrix (weight grad) and of kGroup row tiles
   __nv_bfloat16* out;
-  int wide_stores;  // output rows start on 32-byte boundaries
   int32_t* status;
+  int32_t* taken;  // tiles handed out beyond every pair's first; NULL: pair u walks tiles u, u + pairs, ...
+  int queue;       // ... and how many of them a pair holds at most
 };
+
+constexpr int kQueue = 4;
 
 struct Sched {
   int first[kMaxExperts + 1];  // first row of expert e
   int tiles[kMaxExperts + 1];  // product: tiles before expert e
+  int queue[kQueue];
 };
 
-constexpr int kOffBar = kStages * kStage;
-constexpr int kOffSched = kOffBar + 512;
-constexpr int kSmem = kOffSched + static_cast<int>(sizeof(Sched)) + 1024;
-static_assert(kSmem <= 227 * 1024, "shared memory of expert_linear_kernel");
+template <bool WGRAD>
+struct Config {
+  static constexpr int kGroups = WGRAD ? 2 : 1;  // of epilogue warps
+  static constexpr int kTails = WGRAD ? 2 : 0;
+  static constexpr int kThreads = 128 + kGroups * 128;
+  static constexpr int kOffTail = kStages * kStage;
+  static constexpr int kOffBar = kOffTail + kTails * kTail;
+  static constexpr int kOffSched = kOffBar + 512;
+  static constexpr int kSmem = kOffSched + static_cast<int>(sizeof(Sched)) + 1024;
+  static_assert(kSmem <= 227 * 1024, "shared memory of expert_linear_kernel");
+};
 
 // MN-major tile, 128B swizzle: rows of 64 contiguous outputs, eight contraction steps per 1024 bytes; the second 64
-// outputs follow 64 steps (8192 bytes) later.
-__device__ __forceinline__ uint64_t desc_sw128_mn(uint32_t saddr) {
+// outputs follow `box` bytes later, behind all steps of the first.
+__device__ __forceinline__ uint64_t desc_sw128_mn(uint32_t saddr, uint32_t box = 8192) {
   uint64_t d = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
-  d |= static_cast<uint64_t>(8192 >> 4) << 16;  // leading byte offset: to the next 64 outputs
+  d |= static_cast<uint64_t>(box >> 4) << 16;   // leading byte offset: to the next 64 outputs
   d |= static_cast<uint64_t>(1024 >> 4) << 32;  // stride byte offset: to the next eight contraction steps
   d |= static_cast<uint64_t>(1) << 46;
   d |= static_cast<uint64_t>(2) << 61;
@@ -94,29 +127,44 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
 }
 
 struct Tile {
-  int expert, row0, rows;  // weight grad: the contraction's rows; product: output rows
-  int m0, n0;              // first output row of the tile (weight grad: within the matrix) and column
+  int expert;
+  int row0, rows;  // output rows: of the row matrix (product), of the expert's matrix (weight grad)
+  int c0;          // first output column
+  int k0, k;       // weight grad: the contraction's rows
+  // Steps of 16 that the ring brings (a weight grad's ragged end comes through its own buffer), and slabs of four.
+  template <bool WGRAD>
+  __device__ __forceinline__ int steps() const { return WGRAD ? k >> 4 : (k + 15) >> 4; }
+  template <bool WGRAD>
+  __device__ __forceinline__ int slabs() const { return (steps<WGRAD>() + 3) >> 2; }
 };
 
-// Tiles of a matrix of m_tiles x n_tiles in groups of kGroup row tiles.
-__device__ __forceinline__ void grouped_order(int i, int m_tiles, int n_tiles, int& mt, int& nt) {
-  const int g = i / (kGroup * n_tiles), r = i - g * kGroup * n_tiles;
-  const int width = min(kGroup, m_tiles - g * kGroup);
-  nt = r / width;
-  mt = g * kGroup + r - nt * width;
+// Tiles of a matrix of row_tiles x col_tiles in groups of kGroup row tiles.
+__device__ __forceinline__ void grouped_order(const Params& p, int i, int row_tiles, int& rt, int& ct) {
+  const int g = p.per_group.quotient(i), r = i - g * kGroup * p.col_tiles;
+  const int width = min(kGroup, row_tiles - g * kGroup);
+  if (width == kGroup) {
+    ct = r / kGroup;
+  } else {  // r < 2^23: the product is off by less than one
+    ct = static_cast<int>(static_cast<float>(r) * __frcp_rn(static_cast<float>(width)));
+    const int rest = r - ct * width;
+    ct += rest >= width ? 1 : (rest < 0 ? -1 : 0);
+  }
+  rt = g * kGroup + r - ct * width;
 }
+
+__device__ __forceinline__ int round_up32(int v) { return (v + 31) & ~31; }
 
 template <bool WGRAD>
 __device__ __forceinline__ Tile decode_tile(const Params& p, const Sched& s, int tile) {
   Tile t;
-  int mt, nt;
+  int rt, ct;
   if constexpr (WGRAD) {
-    const int per = p.m_tiles * p.n_tiles;
-    t.expert = tile / per;
-    grouped_order(tile - t.expert * per, p.m_tiles, p.n_tiles, mt, nt);
-    t.row0 = s.first[t.expert];
-    t.rows = s.first[t.expert + 1] - t.row0;
-    t.m0 = mt * 256;
+    t.expert = p.per_matrix.quotient(tile);
+    grouped_order(p, tile - t.expert * p.row_tiles * p.col_tiles, p.row_tiles, rt, ct);
+    t.k0 = s.first[t.expert];
+    t.k = s.first[t.expert + 1] - t.k0;
+    t.row0 = rt * 256;
+    t.rows = min(256, p.rows - t.row0);
   } else {
     int lo = 0, hi = p.E - 1;  // the last expert whose first tile is not behind this one
     while (lo < hi) {
@@ -125,36 +173,80 @@ __device__ __forceinline__ Tile decode_tile(const Params& p, const Sched& s, int
       else hi = mid - 1;
     }
     t.expert = lo;
-    const int first = s.first[lo], end = s.first[lo + 1];
-    grouped_order(tile - s.tiles[lo], (end - first + 255) >> 8, p.n_tiles, mt, nt);
-    t.m0 = 0;
-    t.row0 = first + mt * 256;
-    t.rows = min(256, end - t.row0);
+    const int first = s.first[lo], count = s.first[lo + 1] - first;
+    const int row_tiles = (count + 255) >> 8;
+    grouped_order(p, tile - s.tiles[lo], row_tiles, rt, ct);
+    const int width = round_up32((count + row_tiles - 1) / row_tiles);
+    t.row0 = first + rt * width;
+    t.rows = min(width, count - rt * width);
+    t.k0 = 0;
+    t.k = p.k;
   }
-  t.n0 = nt * 256;
+  t.c0 = ct * 256;
   return t;
 }
 
-// B_MN: the B operand is MN-major (always so for the weight grad, whose A operand is too).
-template <bool WGRAD, bool B_MN>
-__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
-expert_linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const Params p) {
-  constexpr bool A_MN = WGRAD;
+// Arrive at a barrier of the odd CTA, which hands out the tiles.  What it announces is that a load has returned (its value has
+// decided a branch), so it orders nothing: a release would wait for the epilogue's stores.
+__device__ __forceinline__ void mbar_arrive_odd_relaxed(uint64_t* bar) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(bar)), "r"(1));
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+}
+
+// The tiles of a pair, as one warp sees them.
+template <bool QUEUE>
+struct Walk {
+  const Params& p;
+  const Sched& s;
+  uint64_t *full, *empty;  // of the queue's entries: per CTA, in the odd CTA
+  volatile int* abort_flag;
+  int unit, n_units, total, i;
+  // The next tile, -1 behind the last.
+  __device__ __forceinline__ int next() {
+    const int at = i++;
+    if (!QUEUE || p.taken == nullptr || at == 0) {
+      const int64_t tile = unit + static_cast<int64_t>(at) * n_units;
+      return tile < total ? static_cast<int>(tile) : -1;
+    }
+    const int slot = (at - 1) % p.queue;
+    if (!mbar_wait_cluster(&full[slot], (at - 1) / p.queue & 1, abort_flag, p.status, 47)) return -1;
+    const int tile = *static_cast<const volatile int*>(&s.queue[slot]);
+    __syncwarp();
+    if (tile >= total) return -1;
+    if ((threadIdx.x & 31) == 0) mbar_arrive_odd_relaxed(&empty[slot]);
+    return tile;
+  }
+};
+
+// Row boxes of a product: 128, 64, 32 and 16 rows (a tile's half is any multiple of 16).  Weight grad: of the row and the
+// column operand 64 contraction rows in size[0] and the kernel's own column map, 16 in size[2] and size[3].
+struct RowMaps { CUtensorMap size[4]; };
+
+// COL_MN: the column operand is MN-major (always so for the weight grad, whose row operand is too).
+template <bool WGRAD, bool COL_MN>
+__global__ void __launch_bounds__(Config<WGRAD>::kThreads, 1) __cluster_dims__(2, 1, 1)
+expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_constant__ RowMaps row_map, const Params p) {
+  using C = Config<WGRAD>;
+  constexpr int kGroups = C::kGroups, kThreads = C::kThreads;
   constexpr uint32_t kTmemCols = 512;
-  constexpr uint32_t kIdesc = make_idesc_bf16(256, 256) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+  constexpr uint32_t kIdesc = make_idesc_bf16(256, 0) | (COL_MN ? 1u << 15 : 0u) | (WGRAD ? 1u << 16 : 0u);  // N per tile
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* full = bars;
   uint64_t* empty = bars + kStages;
-  uint64_t* tail_full = bars + 2 * kStages;   // a contraction's ragged end landed (per CTA) ...
-  uint64_t* tail_ready = bars + 3 * kStages;  // ... and is cleared in both CTAs (even CTA)
-  uint64_t* tmem_full = bars + 4 * kStages;
-  uint64_t* tmem_empty = bars + 4 * kStages + 2;
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(bars + 4 * kStages + 4);
+  uint64_t* tmem_full = bars + 2 * kStages;
+  uint64_t* tmem_empty = tmem_full + 2;
+  uint64_t* tail_full = tmem_full + 4;   // a ragged end landed (per CTA),
+  uint64_t* tail_ready = tmem_full + 6;  // is cleared in both CTAs (even CTA),
+  uint64_t* tail_empty = tmem_full + 8;  // and has been used
+  uint64_t* queue_full = tmem_full + 10;
+  uint64_t* queue_empty = queue_full + kQueue;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(queue_empty + kQueue);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
-  Sched& s = *reinterpret_cast<Sched*>(smem + kOffSched);
+  Sched& s = *reinterpret_cast<Sched*>(smem + C::kOffSched);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
@@ -164,12 +256,17 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_con
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
-      mbar_init(&tail_full[i], 1);
-      mbar_init(&tail_ready[i], 2);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tmem_full[a], 1);
-      mbar_init(&tmem_empty[a], 16);
+      mbar_init(&tmem_empty[a], 2 * 4 * kGroups);
+      mbar_init(&tail_full[a], 1);
+      mbar_init(&tail_ready[a], 2);
+      mbar_init(&tail_empty[a], 1);
+    }
+    for (int a = 0; a < kQueue; ++a) {
+      mbar_init(&queue_full[a], 1);
+      mbar_init(&queue_empty[a], 2 * (4 * kGroups + 2) + 1);  // every warp that walks the tiles
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -201,7 +298,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_con
       int before = __shfl_up_sync(0xffffffffu, at, 1);
       if (lane == 0) before = e == 0 ? at : top;
       top = __shfl_sync(0xffffffffu, at, 31);
-      int tiles = ((at - before + 255) >> 8) * p.n_tiles;  // of expert e - 1
+      int tiles = ((at - before + 255) >> 8) * p.col_tiles;  // of expert e - 1
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, tiles, o);
@@ -219,52 +316,33 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_con
   cluster_sync_all();  // the peer's barriers exist before anything signals them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr;
-  const int total = WGRAD ? p.E * p.m_tiles * p.n_tiles : s.tiles[p.E];
-  const int k_slabs_fixed = WGRAD ? 0 : (p.k + 63) >> 6;
+  const int total = WGRAD ? p.E * p.row_tiles * p.col_tiles : s.tiles[p.E];
+  Walk<!WGRAD> walk{p, s, queue_full, queue_empty, abort_flag, unit, n_units, total, 0};
 
-  if (warp == 0 || warp == 3) {
-    // ------------------------------------------------------------ producers
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer of the column operand
     const bool leader = elect_one();
-    const bool is_a = warp == 0;
-    const CUtensorMap* map = is_a ? &a_map : &b_map;
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int tile = unit; tile < total && ok; tile += n_units) {
+    for (int tile = walk.next(); tile >= 0 && ok; tile = walk.next()) {
       const Tile t = decode_tile<WGRAD>(p, s, tile);
-      const int slabs = WGRAD ? (t.rows + 63) >> 6 : k_slabs_fixed;
-      const int out0 = (is_a ? (WGRAD ? t.m0 : t.row0) : t.n0) + rank * 128;  // first of this CTA's 128 outputs
+      const int slabs = t.slabs<WGRAD>(), c = t.c0 + rank * 128;
+      // the even CTA's barrier counts both CTAs' bytes
+      const uint32_t bytes = 2 * kOperand + (WGRAD ? 2 * kOperand : round_up32(t.rows) * 128);
       for (int kb = 0; kb < slabs; ++kb) {
         if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, 41)) { ok = false; break; }
-        uint8_t* dst = smem + stage * kStage + (is_a ? 0 : kOperand);
-        const bool ragged = WGRAD && kb == slabs - 1 && (t.rows & 15) != 0;
+        uint8_t* dst = smem + stage * kStage;
         if (leader) {
-          uint64_t* bar = &full[stage];
-          if (ragged) {
-            bar = &tail_full[stage];
-            if (is_a) {
-              mbar_expect_tx(bar, kStage);
-              if (rank == 0) mbar_arrive(&full[stage]);
-            }
-          } else if (is_a && rank == 0) {
-            mbar_expect_tx(bar, 2 * kStage);
-          }
+          if (rank == 0) mbar_expect_tx(&full[stage], bytes);
           if constexpr (WGRAD) {
-            const int r = t.row0 + kb * 64;
-            if (ragged) {
-              tma_load_2d(dst, map, out0, r, bar);
-              tma_load_2d(dst + 8192, map, out0 + 64, r, bar);
-            } else {
-              tma2_load_2d(dst, map, out0, r, bar);
-              tma2_load_2d(dst + 8192, map, out0 + 64, r, bar);
-            }
-          } else if (is_a) {
-            tma2_load_2d(dst, map, kb * 64, out0, bar);
-          } else if constexpr (B_MN) {
-            tma2_load_3d(dst, map, out0, kb * 64, t.expert, bar);
-            tma2_load_3d(dst + 8192, map, out0 + 64, kb * 64, t.expert, bar);
+            tma2_load_2d(dst, &col_map, c, t.k0 + kb * 64, &full[stage]);
+            tma2_load_2d(dst + 8192, &col_map, c + 64, t.k0 + kb * 64, &full[stage]);
+          } else if constexpr (COL_MN) {
+            tma2_load_3d(dst, &col_map, c, kb * 64, t.expert, &full[stage]);
+            tma2_load_3d(dst + 8192, &col_map, c + 64, kb * 64, t.expert, &full[stage]);
           } else {
-            tma2_load_3d(dst, map, kb * 64, out0, t.expert, bar);
+            tma2_load_3d(dst, &col_map, kb * 64, c, t.expert, &full[stage]);
           }
         }
         if (++stage == kStages) { stage = 0; phase ^= 1u; }
@@ -274,138 +352,197 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_con
       // let copies already in flight land before the CTA retires
       for (int i = 0; i < 2000; ++i) __nanosleep(1000);
     }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------ producer of the row operand
+    const bool leader = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = walk.next(); tile >= 0 && ok; tile = walk.next()) {
+      const Tile t = decode_tile<WGRAD>(p, s, tile);
+      const int slabs = t.slabs<WGRAD>();
+      const int half = WGRAD ? 128 : round_up32(t.rows) >> 1;
+      const int r = t.row0 + rank * half;
+      for (int kb = 0; kb < slabs; ++kb) {
+        if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, 41)) { ok = false; break; }
+        uint8_t* dst = smem + stage * kStage + kOperand;
+        if (leader) {
+          if constexpr (WGRAD) {
+            tma2_load_2d(dst, &row_map.size[0], r, t.k0 + kb * 64, &full[stage]);
+            tma2_load_2d(dst + 8192, &row_map.size[0], r + 64, t.k0 + kb * 64, &full[stage]);
+          } else {
+            int at = 0;
+            if (half & 128) { tma2_load_2d(dst, &row_map.size[0], kb * 64, r, &full[stage]); at = 128; }
+            if (half & 64) { tma2_load_2d(dst + at * 128, &row_map.size[1], kb * 64, r + at, &full[stage]); at += 64; }
+            if (half & 32) { tma2_load_2d(dst + at * 128, &row_map.size[2], kb * 64, r + at, &full[stage]); at += 32; }
+            if (half & 16) tma2_load_2d(dst + at * 128, &row_map.size[3], kb * 64, r + at, &full[stage]);
+          }
+        }
+        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    if (!ok) {
+      for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    }
   } else if (warp == 1 && rank == 0) {
     // ------------------------------------------------------------ MMA issuer
     const bool leader = elect_one();
-    int stage = 0, it = 0;
-    uint32_t phase = 0, tail_phase = 0;
+    int stage = 0, it = 0, ends = 0;
+    uint32_t phase = 0;
     bool ok = true;
-    for (int tile = unit; tile < total && ok; tile += n_units) {
-      int rows = 0, slabs = k_slabs_fixed, last = ((p.k + 15) >> 4) - 4 * (slabs - 1);
-      if constexpr (WGRAD) {
-        const int e = tile / (p.m_tiles * p.n_tiles);
-        rows = s.first[e + 1] - s.first[e];
-        if (rows == 0) continue;
-        slabs = (rows + 63) >> 6;
-        last = ((rows + 15) >> 4) - 4 * (slabs - 1);
-      }
+    Tile t;
+    int tile = walk.next();
+    if (tile >= 0) t = decode_tile<WGRAD>(p, s, tile);
+    const auto advance = [&] {
+      tile = walk.next();
+      if (tile >= 0) t = decode_tile<WGRAD>(p, s, tile);
+    };
+    while (tile >= 0 && ok) {
+      const int k = t.k, slabs = t.slabs<WGRAD>(), last = t.steps<WGRAD>() - 4 * (slabs - 1);
+      const uint32_t idesc = kIdesc | (static_cast<uint32_t>((WGRAD ? 256 : round_up32(t.rows)) >> 3) << 17);
+      if (slabs == 0) advance();
+      if (WGRAD && k == 0) continue;
       const int acc = it & 1;
       if (!mbar_wait(&tmem_empty[acc], ((it >> 1) & 1) ^ 1u, abort_flag, p.status, 42)) break;
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + acc * 256;
       for (int kb = 0; kb < slabs; ++kb) {
         if (!mbar_wait(&full[stage], phase, abort_flag, p.status, 43)) { ok = false; break; }
-        if (WGRAD && kb == slabs - 1 && (rows & 15) != 0) {
-          if (!mbar_wait_cluster(&tail_ready[stage], (tail_phase >> stage) & 1u, abort_flag, p.status, 44)) { ok = false; break; }
-          tail_phase ^= 1u << stage;
-        }
         tc_fence_after();
-        const uint32_t sa = smem_u32(smem + stage * kStage), sb = sa + kOperand;
-        const uint64_t a_desc = A_MN ? desc_sw128_mn(sa) : desc_sw128(sa);
-        const uint64_t b_desc = B_MN ? desc_sw128_mn(sb) : desc_sw128(sb);
+        const uint32_t sc = smem_u32(smem + stage * kStage), sr = sc + kOperand;
+        const uint64_t c_desc = COL_MN ? desc_sw128_mn(sc) : desc_sw128(sc);
+        const uint64_t r_desc = WGRAD ? desc_sw128_mn(sr) : desc_sw128(sr);
         if (leader) {
           const int steps = kb == slabs - 1 ? last : 4;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (k < steps)  // 16 contraction steps: 32 bytes along a K-major row, 16 rows of an MN-major tile
-              tc2_mma_bf16(d_tmem, a_desc + k * (A_MN ? 128 : 2), b_desc + k * (B_MN ? 128 : 2), kIdesc, (kb | k) != 0);
+          for (int i = 0; i < 4; ++i) {
+            if (i < steps)  // 16 contraction steps: 32 bytes along a K-major row, 16 rows of an MN-major tile
+              tc2_mma_bf16(d_tmem, c_desc + i * (COL_MN ? 128 : 2), r_desc + i * (WGRAD ? 128 : 2), idesc, (kb | i) != 0);
           }
           tc2_commit_pair(&empty[stage]);
         }
+        if (kb == slabs >> 1) advance();  // while the tensor pipe has work
         if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      }
+      if constexpr (WGRAD) if (ok && (k & 15) != 0) {
+        const int b = ends % C::kTails;
+        if (!mbar_wait_cluster(&tail_ready[b], ends / C::kTails & 1, abort_flag, p.status, 44)) break;
+        tc_fence_after();
+        const uint32_t sc = smem_u32(smem + C::kOffTail + b * kTail);
+        if (leader) {
+          tc2_mma_bf16(d_tmem, desc_sw128_mn(sc, 2048), desc_sw128_mn(sc + 4096, 2048), idesc, slabs != 0);
+          tc2_commit_pair(&tail_empty[b]);
+        }
+        ++ends;
       }
       if (ok && leader) tc2_commit_pair(&tmem_full[acc]);
       ++it;
     }
-  } else if (WGRAD && warp == 2) {
-    // ------------------------------------------------------------ ragged ends
-    int stage = 0;
-    uint32_t tail_phase = 0;
-    bool ok = true;
-    for (int tile = unit; tile < total && ok; tile += n_units) {
-      const int e = tile / (p.m_tiles * p.n_tiles);
-      const int rows = s.first[e + 1] - s.first[e];
-      const int slabs = (rows + 63) >> 6;
-      const int at = (stage + slabs - 1) % kStages;
-      if ((rows & 15) != 0) {
-        if (!mbar_wait(&tail_full[at], (tail_phase >> at) & 1u, abort_flag, p.status, 45)) { ok = false; break; }
-        tail_phase ^= 1u << at;
-        const int from = (rows - 1) % 64 + 1, to = (from + 15) & ~15;  // rows of the slab to clear
-        uint8_t* base = smem + at * kStage;
-        // four boxes (two of either operand) of 64 rows of 128 bytes: 32 lanes clear 512 bytes of a row
-        for (int r = from; r < to; ++r)
-          *reinterpret_cast<uint4*>(base + (lane >> 3) * 8192 + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive_leader(&tail_ready[at]);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ tiles: one ticket after the other, for both CTAs
+    if (!WGRAD && p.taken != nullptr && lane == 0) {
+      for (int i = 0, tile = 0; tile < total; ++i) {
+        const int slot = i % p.queue;
+        if (!mbar_wait_cluster(&queue_empty[slot], (i / p.queue & 1) ^ 1u, abort_flag, p.status, 48)) break;
+        tile = n_units + atomicAdd(p.taken, 1);
+        *static_cast<volatile int*>(&s.queue[slot]) = tile;
+        uint32_t remote;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(&s.queue[slot])), "r"(0));
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(tile) : "memory");
+        mbar_arrive(&queue_full[slot]);
+        mbar_arrive_leader(&queue_full[slot]);
       }
-      stage = (stage + slabs) % kStages;
+    }
+    __syncwarp();
+  } else if (WGRAD && warp == 2) {
+    if constexpr (WGRAD) {
+    // ------------------------------------------------------------ ragged ends
+    const bool leader = elect_one();
+    int ends = 0;
+    for (int tile = walk.next(); tile >= 0; tile = walk.next()) {
+      const Tile t = decode_tile<WGRAD>(p, s, tile);
+      const int rest = t.k & 15;
+      if (rest == 0) continue;
+      const int b = ends % C::kTails;
+      uint8_t* base = smem + C::kOffTail + b * kTail;
+      if (!mbar_wait(&tail_empty[b], (ends / C::kTails & 1) ^ 1u, abort_flag, p.status, 45)) break;
+      if (leader) {
+        const int c = t.c0 + rank * 128, r = t.row0 + rank * 128, k = t.k0 + (t.k & ~15);
+        mbar_expect_tx(&tail_full[b], kTail);
+        tma_load_2d(base, &row_map.size[3], c, k, &tail_full[b]);
+        tma_load_2d(base + 2048, &row_map.size[3], c + 64, k, &tail_full[b]);
+        tma_load_2d(base + 4096, &row_map.size[2], r, k, &tail_full[b]);
+        tma_load_2d(base + 6144, &row_map.size[2], r + 64, k, &tail_full[b]);
+      }
+      __syncwarp();
+      if (!mbar_wait(&tail_full[b], ends / C::kTails & 1, abort_flag, p.status, 45)) {
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+        break;
+      }
+      // 32 lanes clear 512 bytes: a row of all four boxes
+      for (int r = rest; r < 16; ++r)
+        *reinterpret_cast<uint4*>(base + (lane >> 3) * 2048 + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_leader(&tail_ready[b]);
+      ++ends;
+    }
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
-    const int q = warp & 3, half = (warp - 4) >> 2;
-    const int lane_row = rank * 128 + q * 32 + lane;
+    const int q = warp & 3, group = (warp - 4) >> 2;
     int it = 0;
     if constexpr (!WGRAD) {
       // rows of no expert
       const int lo = s.first[0], hi = s.first[p.E], none = lo + p.R - hi;
-      for (int i = blockIdx.x * 8 + warp - 4; i < none; i += gridDim.x * 8) {
-        uint4* row = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(i < lo ? i : i - lo + hi) * p.n);
-        for (int c = lane; c < p.n >> 3; c += 32) row[c] = make_uint4(0, 0, 0, 0);
+      for (int i = blockIdx.x * 4 * kGroups + warp - 4; i < none; i += gridDim.x * 4 * kGroups) {
+        uint4* row = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(i < lo ? i : i - lo + hi) * p.cols);
+        for (int c = lane; c < p.cols >> 3; c += 32) row[c] = make_uint4(0, 0, 0, 0);
       }
     }
-    for (int tile = unit; tile < total; tile += n_units) {
+    for (int tile = walk.next(); tile >= 0; tile = walk.next()) {
       const Tile t = decode_tile<WGRAD>(p, s, tile);
-      const bool live = WGRAD ? t.m0 + lane_row < p.m : lane_row < t.rows;
-      const int64_t out_row = WGRAD ? static_cast<int64_t>(t.expert) * p.m + t.m0 + lane_row : t.row0 + lane_row;
-      const int c0 = t.n0 + half * 128;
-      __nv_bfloat16* out = p.out + out_row * p.n + c0;
-      const int cols = min(128, p.n - c0);
-      const bool empty_tile = WGRAD && t.rows == 0;
-      const int acc = it & 1;
-      if (!empty_tile) {
-        if (!mbar_wait(&tmem_full[acc], (it >> 1) & 1, abort_flag, p.status, 46)) break;
-        __syncwarp();
-        tc_fence_after();
-        ++it;
+      const int64_t row0 = (WGRAD ? static_cast<int64_t>(t.expert) * p.rows : 0) + t.row0;
+      if (WGRAD && t.k == 0) {  // an expert without rows: zeros, eight columns per thread
+        const int c = t.c0 + rank * 128 + (lane & 15) * 8;
+        for (int r = (warp - 4) * 2 + (lane >> 4); r < t.rows && c < p.cols; r += 8 * kGroups)
+          *reinterpret_cast<uint4*>(p.out + (row0 + r) * p.cols + c) = make_uint4(0, 0, 0, 0);
+        continue;
       }
-      const uint32_t taddr = tmem_base + acc * 256 + half * 128 + (static_cast<uint32_t>(q * 32) << 16);
-#pragma unroll
-      for (int c = 0; c < 128; c += 32) {
+      const int col = t.c0 + rank * 128 + q * 32 + lane;
+      const int acc = it & 1;
+      if (!mbar_wait(&tmem_full[acc], (it >> 1) & 1, abort_flag, p.status, 46)) break;
+      __syncwarp();
+      tc_fence_after();
+      ++it;
+      const uint32_t taddr = tmem_base + acc * 256 + (static_cast<uint32_t>(q * 32) << 16);
+      const int chunks = (t.rows + 31) >> 5;
+      // also a group without a chunk in this tile has to hand the accumulator back
+      if (group >= chunks && lane == 0) mbar_arrive_leader_relaxed(&tmem_empty[acc]);
+      __nv_bfloat16* out = p.out + (row0 + group * 32) * p.cols + col;
+      for (int c = group; c < chunks; c += kGroups) {
         uint32_t v[32];
-        if (empty_tile) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0;
-        } else {
-          tc_ld32_nowait(taddr + c, v);
-          tc_wait_ld();
+        tc_ld32_nowait(taddr + c * 32, v);
+        tc_wait_ld();
+        if (c + kGroups >= chunks) {  // the group's last look at this accumulator
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_leader_relaxed(&tmem_empty[acc]);
         }
-        if (live) {
-          uint32_t w[16];
+        const int rows = min(32, t.rows - c * 32);
+        if (col < p.cols) {
+          __nv_bfloat16* o = out;
+          if (rows == 32) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-            w[j] = *reinterpret_cast<const uint32_t*>(&b);
-          }
-          if (p.wide_stores) {  // n and with it every part that is left is a multiple of 16 columns
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              if (c + j * 16 < cols)
-                st_global_256(out + c + j * 16, w[8 * j], w[8 * j + 1], w[8 * j + 2], w[8 * j + 3], w[8 * j + 4],
-                              w[8 * j + 5], w[8 * j + 6], w[8 * j + 7]);
+            for (int j = 0; j < 32; ++j, o += p.cols) *o = __float2bfloat16_rn(__uint_as_float(v[j]));
           } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (c + j * 8 < cols)
-                *reinterpret_cast<uint4*>(out + c + j * 8) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+            for (int j = 0; j < 32; ++j, o += p.cols)
+              if (j < rows) *o = __float2bfloat16_rn(__uint_as_float(v[j]));
           }
         }
-        __syncwarp();  // the next load wants the whole warp
-      }
-      if (!empty_tile) {
-        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_leader_relaxed(&tmem_empty[acc]);
+        out += static_cast<int64_t>(kGroups) * 32 * p.cols;
       }
     }
   }
@@ -436,13 +573,13 @@ int make_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int
   return B200MOE_OK;
 }
 
-template <bool WGRAD, bool B_MN>
-int launch(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int64_t tiles, cudaStream_t st) {
-  auto kern = expert_linear_kernel<WGRAD, B_MN>;
-  B200MOE_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), kSmem));
+template <bool WGRAD, bool COL_MN>
+int launch(const CUtensorMap& cols, const RowMaps& rows, const Params& p, int64_t tiles, cudaStream_t st) {
+  auto kern = expert_linear_kernel<WGRAD, COL_MN>;
+  B200MOE_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), Config<WGRAD>::kSmem));
   const int64_t units = sm_count() / 2;
-  B200MOE_CUDA_OK(launch_overlapped(kern, dim3(static_cast<unsigned>(2 * (tiles < units ? tiles : units))), kThreads, kSmem,
-                                    st, a, b, p));
+  B200MOE_CUDA_OK(launch_overlapped(kern, dim3(static_cast<unsigned>(2 * (tiles < units ? tiles : units))), Config<WGRAD>::kThreads,
+                                    Config<WGRAD>::kSmem, st, cols, rows, p));
   B200MOE_LAUNCH_OK("expert_linear_kernel");
   return B200MOE_OK;
 }
@@ -475,21 +612,33 @@ extern "C" int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch,
   p.offsets = expert_offsets;
   p.R = R;
   p.E = E;
-  p.n = n;
+  p.cols = n;
   p.k = k;
-  p.n_tiles = (n + 255) / 256;
+  p.col_tiles = (n + 255) / 256;
+  B200MOE_REQUIRE(p.col_tiles < (1 << 20), B200MOE_ERR_INVALID, "expert_product: too many output columns");
+  p.per_matrix = p.per_group = make_divisor(static_cast<uint32_t>(kGroup * p.col_tiles));
   p.out = static_cast<__nv_bfloat16*>(out_bf16);
-  p.wide_stores = n % 16 == 0 && (reinterpret_cast<uintptr_t>(out_bf16) & 31) == 0;
   p.status = status;
-  const int64_t most_tiles = (ceil_div64(R, 256) + (E < R ? E : R)) * p.n_tiles;
+  const int64_t most_tiles = (ceil_div64(R, 256) + (E < R ? E : R)) * p.col_tiles;
   B200MOE_REQUIRE(most_tiles < (int64_t{1} << 30), B200MOE_ERR_INVALID, "expert_product: too many output tiles");
-  CUtensorMap a, b;
-  int rc = make_map(&a, rows_bf16, k, R, rows_pitch, 0, 0, 128);
-  if (rc != B200MOE_OK) return rc;
-  rc = make_map(&b, weight_bf16, D1, D0, w_pitch, E, w_expert_pitch, contract_last ? 128 : 64);
+  CUtensorMap cols;
+  RowMaps rows;
+  int rc = make_map(&cols, weight_bf16, D1, D0, w_pitch, E, w_expert_pitch, contract_last ? 128 : 64);
+  for (int i = 0; i < 4 && rc == B200MOE_OK; ++i) rc = make_map(&rows.size[i], rows_bf16, k, R, rows_pitch, 0, 0, 128 >> i);
   if (rc != B200MOE_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return contract_last ? launch<false, false>(a, b, p, most_tiles, st) : launch<false, true>(a, b, p, most_tiles, st);
+  // Row tiles of an expert share its weight tiles in L2 as long as they run side by side.  A fixed walk drifts apart, since
+  // tiles differ in width; handed out in order as pairs come free they stay together (32 experts of 7168 x 4096, 32768
+  // rows, skewed: 5.6 -> 2.8 GB from DRAM, 1533 -> 1356 us; its row gradient 3.6 -> 2.4 GB, 1440 -> 1342 us).  With one row
+  // tile per expert there is nothing to share, and the counter's memset and the queue cost more than they bring (64 experts
+  // of 2048 x 2048, 125 rows each: 109 us without, 118 with); so they do for the weight gradient's short contractions (4 x 1024
+  // rows, 4096 x 14336: 353 and 367 us).
+  if (R >= 512 * static_cast<int64_t>(E) && most_tiles >= 4 * (sm_count() / 2)) {
+    p.taken = status + 1;
+    p.queue = k >= 1024 ? 2 : kQueue;
+    B200MOE_CUDA_OK(cudaMemsetAsync(p.taken, 0, sizeof(int32_t), st));
+  }
+  return contract_last ? launch<false, false>(cols, rows, p, most_tiles, st) : launch<false, true>(cols, rows, p, most_tiles, st);
 }
 
 extern "C" int b200moe_expert_weight_grad(const void* a_bf16, int64_t a_pitch, const void* b_bf16, int64_t b_pitch,
@@ -509,19 +658,24 @@ extern "C" int b200moe_expert_weight_grad(const void* a_bf16, int64_t a_pitch, c
   p.offsets = expert_offsets;
   p.R = R;
   p.E = E;
-  p.m = M;
-  p.n = N;
-  p.m_tiles = (M + 255) / 256;
-  p.n_tiles = (N + 255) / 256;
+  p.rows = M;
+  p.cols = N;
+  p.row_tiles = (M + 255) / 256;
+  p.col_tiles = (N + 255) / 256;
   p.out = static_cast<__nv_bfloat16*>(out_bf16);
-  p.wide_stores = N % 16 == 0 && (reinterpret_cast<uintptr_t>(out_bf16) & 31) == 0;
   p.status = status;
-  const int64_t tiles = static_cast<int64_t>(E) * p.m_tiles * p.n_tiles;
+  const int64_t tiles = static_cast<int64_t>(E) * p.row_tiles * p.col_tiles;
+  B200MOE_REQUIRE(p.col_tiles < (1 << 20), B200MOE_ERR_INVALID, "expert_weight_grad: too many output columns");
   B200MOE_REQUIRE(tiles < (int64_t{1} << 30), B200MOE_ERR_INVALID, "expert_weight_grad: too many output tiles");
-  CUtensorMap a, b;
-  int rc = make_map(&a, a_bf16, M, R, a_pitch, 0, 0, 64);
+  p.per_matrix = make_divisor(static_cast<uint32_t>(p.row_tiles * p.col_tiles));
+  p.per_group = make_divisor(static_cast<uint32_t>(kGroup * p.col_tiles));
+  CUtensorMap cols;
+  RowMaps rows;
+  int rc = make_map(&cols, b_bf16, N, R, b_pitch, 0, 0, 64);
+  if (rc == B200MOE_OK) rc = make_map(&rows.size[0], a_bf16, M, R, a_pitch, 0, 0, 64);
+  if (rc == B200MOE_OK) rc = make_map(&rows.size[2], a_bf16, M, R, a_pitch, 0, 0, 16);
+  if (rc == B200MOE_OK) rc = make_map(&rows.size[3], b_bf16, N, R, b_pitch, 0, 0, 16);
   if (rc != B200MOE_OK) return rc;
-  rc = make_map(&b, b_bf16, N, R, b_pitch, 0, 0, 64);
-  if (rc != B200MOE_OK) return rc;
-  return launch<true, true>(a, b, p, tiles, static_cast<cudaStream_t>(stream));
+  rows.size[1] = rows.size[0];  // never used
+  return launch<true, true>(cols, rows, p, tiles, static_cast<cudaStream_t>(stream));
 }

@@ -221,6 +221,13 @@ def test_products(counts, K, N, behind, transposed):
     _check_product(COUNTS[counts], K, N, behind, K + N, transposed)
 
 
+@pytest.mark.parametrize("K,N", [(72, 7688), (1032, 7680), (64, 15000)])
+def test_products_whose_tiles_are_handed_out(K, N):
+    """Enough rows per expert and tiles for the pairs to draw their tiles from one counter."""
+    _check_product([3000, 0, 700, 1, 1299], K, N, 40, K, False)
+    _check_product([3000, 0, 700, 1, 1299], N, K, 0, N, True)
+
+
 @pytest.mark.parametrize("rest", range(0, 64, 3))
 def test_weight_gradient_ends_anywhere_in_a_slab(rest):
     """The next expert's rows are inf: none of them may reach this expert's sums."""
