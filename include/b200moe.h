@@ -398,15 +398,18 @@ int b200moe_ep_return_rows(const void* y_pos_bf16, const int32_t* row_valid, con
  * No counterpart in the reference's inference kernels.  Rows are sorted by expert without padding: expert e owns rows expert_offsets[e] to expert_offsets[e + 1] (int32 [E + 1], on the device) of R = T * K rows, E <= 1024.
  *
  * sort_pairs: order of the pairs p = t * K + k of expert_index [T, K] (index_bytes 4 or 8) by (expert, p).  row_of_pair [T, K]
- * gets a pair's row, -1 where the id lies outside [0, E); pair_of_row [T * K] the pair of a row, -1 behind the last expert. */
+ * gets a pair's row, -1 where the id lies outside [0, E).  Up to 2048 pairs need no workspace. */
 size_t b200moe_sort_workspace_bytes(int64_t pairs, int E);
 int b200moe_sort_pairs(const void* expert_index, int index_bytes, int T, int K, int E, int32_t* expert_offsets,
-                       int32_t* row_of_pair, int32_t* pair_of_row, void* workspace, size_t workspace_bytes,
-                       b200moe_stream_t stream);
+                       int32_t* row_of_pair, void* workspace, size_t workspace_bytes, b200moe_stream_t stream);
 /* rows[row_of_pair[t, k]] = hidden[t]; rows behind the last expert become zero.  dtype F32 or BF16, pitches in elements;
  * outputs are contiguous. */
 int b200moe_sort_rows(const void* hidden, int dtype, int64_t pitch, int T, int K, int H, int E,
                       const int32_t* row_of_pair, const int32_t* expert_offsets, void* rows, b200moe_stream_t stream);
+/* sort_pairs and sort_rows in one call. */
+int b200moe_sort_tokens(const void* hidden, int dtype, int64_t pitch, const void* expert_index, int index_bytes, int T, int K,
+                        int H, int E, int32_t* expert_offsets, int32_t* row_of_pair, void* rows, void* workspace,
+                        size_t workspace_bytes, b200moe_stream_t stream);
 /* out[t] = sum over k of affinities[t, k] rows[row_of_pair[t, k]] in fp32, k ascending, one rounding.  affinities [T, K]
  * (aff_dtype) or NULL = 1, which makes it the gradient of sort_rows. */
 int b200moe_unsort_rows(const void* rows, int dtype, int64_t pitch, int T, int K, int H, const int32_t* row_of_pair,

@@ -7,21 +7,25 @@ from typing import Tuple
 import torch
 
 from .... import _lib
-from .launch import launch, needs_grad, pitch_of, same_device, tile_rows
+from .launch import launch, needs_grad, once, pitch_of, refuse, same_device, tile_rows
 from .sort_tokens import MAX_EXPERTS
+
+
+def _readable(w: torch.Tensor) -> bool:
+    """Matrices the kernels can read: contiguous columns, rows and matrices apart and on 16-byte boundaries."""
+    E, rows, cols = w.shape
+    matrix, pitch, unit = w.stride()
+    return (unit == 1 and w.data_ptr() % 16 == 0 and (rows == 1 or pitch >= cols and pitch % 8 == 0) and
+            (E == 1 or matrix >= cols and matrix % 8 == 0))
 
 
 def _stored(weight: torch.Tensor) -> Tuple[torch.Tensor, bool]:
     """``weight [E, K, N]`` as matrices the kernels can read: (tensor, transposed).  Transposed ones lie in memory as
     [E, N, K], like the weights of linear layers; anything else is copied."""
-    def readable(w):
-        pitches = ([w.stride(1)] if w.shape[1] > 1 else []) + ([w.stride(0)] if w.shape[0] > 1 else [])
-        return w.stride(2) == 1 and w.data_ptr() % 16 == 0 and all(p >= w.shape[2] and p % 8 == 0 for p in pitches)
-
-    if readable(weight):
+    if _readable(weight):
         return weight, False
     turned = weight.transpose(1, 2)
-    if readable(turned):
+    if _readable(turned):
         return turned, True
     return weight.clone(memory_format=torch.contiguous_format), False
 
@@ -76,7 +80,7 @@ class _ExpertLinear(torch.autograd.Function):
         return product(rows, weight, expert_offsets, check_status=check_status)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, d_out):
         rows, weight, offsets = ctx.saved_tensors
         d_out = tile_rows(d_out)
@@ -86,16 +90,22 @@ class _ExpertLinear(torch.autograd.Function):
 
 
 def check_rows_and_weight(rows: torch.Tensor, weight: torch.Tensor, expert_offsets: torch.Tensor, name: str) -> None:
-    A = _lib.kernel_assert
-    A(rows.dim() == 2 and rows.dtype == torch.bfloat16, "rows must be bfloat16 [R, K]")
-    A(weight.dim() == 3 and weight.dtype == torch.bfloat16, f"{name} must be bfloat16 with one matrix per expert")
+    if rows.dim() != 2 or rows.dtype != torch.bfloat16:
+        refuse("rows must be bfloat16 [R, K]")
+    if weight.dim() != 3 or weight.dtype != torch.bfloat16:
+        refuse(f"{name} must be bfloat16 with one matrix per expert")
     E, K, N = weight.shape
-    A(rows.shape[1] == K, f"rows have {rows.shape[1]} columns, {name} contracts {K}")
-    A(K > 0 and N > 0 and K % 8 == 0 and N % 8 == 0, f"both sizes of {name}'s matrices ({K}, {N}) must be multiples of 8")
-    A(1 <= E <= MAX_EXPERTS, f"between 1 and {MAX_EXPERTS} experts, got {E}")
-    A(expert_offsets.dtype == torch.int32 and expert_offsets.dim() == 1 and expert_offsets.is_contiguous() and
-      expert_offsets.numel() == E + 1, f"expert_offsets must be int32 [E + 1] = [{E + 1}]")
-    A(rows.shape[0] < 2 ** 31, "at most 2^31 - 1 rows")
+    R, cols = rows.shape
+    if cols != K:
+        refuse(f"rows have {cols} columns, {name} contracts {K}")
+    if K % 8 or N % 8 or not K or not N:
+        refuse(f"both sizes of {name}'s matrices ({K}, {N}) must be multiples of 8")
+    if not 1 <= E <= MAX_EXPERTS:
+        refuse(f"between 1 and {MAX_EXPERTS} experts, got {E}")
+    if expert_offsets.dtype != torch.int32 or expert_offsets.shape != (E + 1,) or not expert_offsets.is_contiguous():
+        refuse(f"expert_offsets must be int32 [E + 1] = [{E + 1}]")
+    if R >= 2 ** 31:
+        refuse("at most 2^31 - 1 rows")
 
 
 def expert_linear(rows: torch.Tensor, weight: torch.Tensor, expert_offsets: torch.Tensor,

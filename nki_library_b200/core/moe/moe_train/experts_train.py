@@ -7,7 +7,7 @@ import torch
 from .... import _lib
 from ...utils.common_types import ActFnType
 from .expert_linear import check_rows_and_weight, product, weight_grad
-from .launch import needs_grad, same_device, tile_rows
+from .launch import needs_grad, once, same_device, tile_rows
 from .moe_glu import glu_backward, glu_forward
 from .sort_tokens import moe_sort_tokens, moe_unsort_tokens
 
@@ -15,20 +15,19 @@ from .sort_tokens import moe_sort_tokens, moe_unsort_tokens
 class _ExpertMLP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, gate_up_weight, down_weight, expert_offsets, act):
-        m, codes, scales = glu_forward(product(rows, gate_up_weight, expert_offsets), act, True)
-        ctx.save_for_backward(rows if gate_up_weight.requires_grad else None, gate_up_weight, down_weight, expert_offsets,
-                              codes, scales)
+        m, kept = glu_forward(product(rows, gate_up_weight, expert_offsets), act, True)
+        ctx.save_for_backward(rows if gate_up_weight.requires_grad else None, gate_up_weight, down_weight, expert_offsets, kept)
         ctx.act = act
         return product(m, down_weight, expert_offsets)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, d_out):
-        rows, gate_up_weight, down_weight, offsets, codes, scales = ctx.saved_tensors
+        rows, gate_up_weight, down_weight, offsets, kept = ctx.saved_tensors
         want_rows, want_gate_up, want_down = ctx.needs_input_grad[:3]
         d_out = tile_rows(d_out)
         d_m = product(d_out, down_weight, offsets, transpose=True)
-        d_gate_up, m = glu_backward(d_m, codes, scales, ctx.act, want_m=want_down)
+        d_gate_up, m = glu_backward(d_m, kept, ctx.act, want_m=want_down)
         d_down = weight_grad(m, d_out, down_weight, offsets) if want_down else None
         d_rows = product(d_gate_up, gate_up_weight, offsets, transpose=True) if want_rows else None
         d_gate_up_weight = weight_grad(rows, d_gate_up, gate_up_weight, offsets) if want_gate_up else None

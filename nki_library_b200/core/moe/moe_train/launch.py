@@ -1,4 +1,8 @@
-"""What the operators of the training pass share: the device and stream of a call, and rows the kernels can read."""
+"""What the operators of the training pass share: the device and stream of a call, and rows the kernels can read.
+
+A call on a few rows is host work: refusals format their messages only when they refuse, and the stream's handle is asked for
+without an object around it (3 us each, four to ten times per training step).
+"""
 
 from __future__ import annotations
 
@@ -6,28 +10,51 @@ import torch
 
 from .... import _lib
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
-def same_device(*tensors) -> torch.device:
-    _lib.require_cuda(*tensors)
-    device = None
-    for t in tensors:
-        if t is not None:
-            _lib.kernel_assert(device is None or t.device == device, "all tensors must live on the same device")
-            device = t.device
+
+def refuse(message: str) -> None:
+    _lib.kernel_assert(False, message)
+
+
+def same_device(first: torch.Tensor, *others) -> torch.device:
+    """The CUDA device that all tensors (or None) live on."""
+    device = first.device
+    if device.type != "cuda":
+        _lib.require_cuda(first)
+    for t in others:
+        if t is not None and t.device != device:
+            _lib.require_cuda(t)
+            refuse("all tensors must live on the same device")
     return device
 
 
 def launch(device: torch.device, name: str, *args) -> None:
     """Call an entry point on the current stream of ``device``, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args, _raw_stream(index))
         return
     with torch.cuda.device(device):
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+        _lib.call(name, *args, _raw_stream(index))
 
 
 def needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def once(backward):
+    """``once_differentiable`` for the one case it is there for, a backward pass that is itself recorded
+    (``create_graph=True``); the usual one does without its bookkeeping."""
+    recorded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def pitch_of(t: torch.Tensor) -> int:
@@ -37,12 +64,13 @@ def pitch_of(t: torch.Tensor) -> int:
 
 def unit_rows(t: torch.Tensor) -> torch.Tensor:
     """``t [rows, cols]`` itself if its columns are contiguous, else a copy."""
-    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
 def tile_rows(t: torch.Tensor) -> torch.Tensor:
     """``t [rows, cols]`` itself if its rows do not overlap and all start on 16-byte boundaries, else a copy."""
-    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (
-            t.shape[0] <= 1 or (t.stride(0) >= t.shape[1] and t.stride(0) * t.element_size() % 16 == 0)):
-        return t
+    if t.data_ptr() % 16 == 0 and t.stride(1) == 1:
+        pitch = t.stride(0)
+        if (pitch >= t.shape[1] and pitch * t.element_size() % 16 == 0) or t.shape[0] <= 1:
+            return t
     return t.clone(memory_format=torch.contiguous_format)

@@ -8,24 +8,30 @@ import torch
 
 from .... import _lib
 from ...utils.common_types import ActFnType
-from .launch import launch, needs_grad, pitch_of, same_device, tile_rows
+from .launch import launch, needs_grad, once, pitch_of, refuse, tile_rows
 
 
-def glu_forward(gate_up: torch.Tensor, act: int, keep: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
-    """``(m, codes, scales)``; the last two None unless ``keep``."""
-    R, I = gate_up.shape[0], gate_up.shape[1] // 2
+def glu_forward(gate_up: torch.Tensor, act: int, keep: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``(m, kept)``; ``kept`` (the codes of all rows, then their scales) None unless ``keep``."""
+    R, two_I = gate_up.shape
+    I = two_I // 2
     device = gate_up.device
     m = torch.empty((R, I), dtype=torch.bfloat16, device=device)
-    codes = torch.empty((R, 2 * I), dtype=torch.uint8, device=device) if keep else None
-    scales = torch.empty((R, 2, (I + 31) // 32), dtype=torch.uint8, device=device) if keep else None
+    kept = torch.empty(R * (two_I + 2 * ((I + 31) // 32)), dtype=torch.uint8, device=device) if keep else None
     if R:
         gate_up = tile_rows(gate_up)
-        launch(device, "b200moe_glu", gate_up.data_ptr(), pitch_of(gate_up), R, I, act, m.data_ptr(), _lib.ptr(codes),
-               _lib.ptr(scales))
-    return m, codes, scales
+        codes = kept.data_ptr() if keep else None
+        launch(device, "b200moe_glu", gate_up.data_ptr(), pitch_of(gate_up), R, I, act, m.data_ptr(), codes,
+               codes + R * two_I if keep else None)
+    return m, kept
 
 
-def glu_backward(d_m: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, act: int,
+def kept_parts(kept: torch.Tensor, R: int, I: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The codes ``[R, 2 I]`` and scales ``[R, 2, ceil(I / 32)]`` of a checkpoint."""
+    return kept[:R * 2 * I].view(R, 2 * I), kept[R * 2 * I:].view(R, 2, (I + 31) // 32)
+
+
+def glu_backward(d_m: torch.Tensor, kept: torch.Tensor, act: int,
                  want_m: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``(d_gate_up, m)`` at the kept gate and up; ``m`` None unless wanted."""
     R, I = d_m.shape
@@ -33,24 +39,25 @@ def glu_backward(d_m: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, a
     m = torch.empty((R, I), dtype=torch.bfloat16, device=d_m.device) if want_m else None
     if R:
         d_m = tile_rows(d_m)
-        launch(d_m.device, "b200moe_glu_backward", d_m.data_ptr(), pitch_of(d_m), codes.data_ptr(), scales.data_ptr(), R, I,
-               act, d_gate_up.data_ptr(), _lib.ptr(m))
+        codes = kept.data_ptr()
+        launch(d_m.device, "b200moe_glu_backward", d_m.data_ptr(), pitch_of(d_m), codes, codes + R * 2 * I, R, I, act,
+               d_gate_up.data_ptr(), _lib.ptr(m))
     return d_gate_up, m
 
 
 class _Glu(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate_up, act):
-        m, codes, scales = glu_forward(gate_up, act, True)
-        ctx.save_for_backward(codes, scales)
+        m, kept = glu_forward(gate_up, act, True)
+        ctx.save_for_backward(kept)
         ctx.act = act
         return m
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, d_m):
-        codes, scales = ctx.saved_tensors
-        return glu_backward(d_m, codes, scales, ctx.act)[0], None
+        kept, = ctx.saved_tensors
+        return glu_backward(d_m, kept, ctx.act)[0], None
 
 
 def moe_glu(gate_up: torch.Tensor, activation_function: ActFnType = ActFnType.SiLU) -> torch.Tensor:
@@ -61,14 +68,16 @@ def moe_glu(gate_up: torch.Tensor, activation_function: ActFnType = ActFnType.Si
     is off by at most 2^-4 of itself, or 2^-10 of the power).  The gradient is the formula's at the kept values.  Values that
     are not finite are kept as NaN and leave their neighbours' scale alone.  I is a multiple of 8.
     """
-    _lib.require_cuda(gate_up)
-    A = _lib.kernel_assert
-    A(gate_up.dtype == torch.bfloat16 and (gate_up.dim() == 2 or gate_up.dim() == 3 and gate_up.shape[1] == 2),
-      "gate_up must be bfloat16 [R, 2 I] or [R, 2, I]")
-    A(isinstance(activation_function, ActFnType), "activation_function must be an ActFnType")
-    if gate_up.dim() == 3:
+    if not gate_up.is_cuda:
+        _lib.require_cuda(gate_up)
+    if gate_up.dim() == 3 and gate_up.shape[1] == 2:
         gate_up = gate_up.flatten(1)
-    A(gate_up.shape[1] > 0 and gate_up.shape[1] % 16 == 0, f"I must be a multiple of 8, gate_up has {gate_up.shape[1]} columns")
+    if gate_up.dtype != torch.bfloat16 or gate_up.dim() != 2:
+        refuse("gate_up must be bfloat16 [R, 2 I] or [R, 2, I]")
+    if not isinstance(activation_function, ActFnType):
+        refuse("activation_function must be an ActFnType")
+    if gate_up.shape[1] == 0 or gate_up.shape[1] % 16:
+        refuse(f"I must be a multiple of 8, gate_up has {gate_up.shape[1]} columns")
     if needs_grad(gate_up):
         return _Glu.apply(gate_up, activation_function.value)
     return glu_forward(gate_up, activation_function.value, False)[0]

@@ -7,73 +7,83 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from .... import _lib
-from .launch import launch, needs_grad, pitch_of, same_device, unit_rows
+from .launch import launch, needs_grad, once, pitch_of, refuse, same_device, unit_rows
 
 MAX_EXPERTS = 1024
+_ID_TYPES = (torch.int32, torch.uint32, torch.int64)
+_ONE_LAUNCH = 2048  # pairs that the sort takes without a workspace
 
 
 class SortedTokens(NamedTuple):
-    """The order of the T * K (token, choice) pairs by (expert, token, choice), all int32 on the device.
+    """The order of the T * K (token, choice) pairs by (expert, token, choice), int32 on the device.
 
     Expert e owns rows ``expert_offsets[e]`` to ``expert_offsets[e + 1]``; pair (t, k) sits in row ``row_of_pair[t, k]``, or
-    in none (-1) if its expert id lies outside ``[0, num_experts)``; row r holds pair ``pair_of_row[r]`` = t * K + k, or none
-    (-1) behind the last expert.
+    in none (-1) if its expert id lies outside ``[0, num_experts)``.
     """
     expert_offsets: torch.Tensor
     row_of_pair: torch.Tensor
-    pair_of_row: torch.Tensor
     num_experts: int
+
+
+def _sort(expert_index: torch.Tensor, num_experts: int, hidden: Optional[torch.Tensor]):
+    """``(rows, plan)``; rows None without ``hidden``."""
+    if not expert_index.is_cuda:
+        _lib.require_cuda(expert_index)
+    if expert_index.dim() != 2:
+        refuse("expert_index must be [T, K]")
+    if expert_index.dtype not in _ID_TYPES:
+        refuse("expert_index must be int32, uint32 or int64")
+    E = int(num_experts)
+    if not 1 <= E <= MAX_EXPERTS:
+        refuse(f"num_experts ({num_experts}) must be between 1 and {MAX_EXPERTS}")
+    T, K = expert_index.shape
+    pairs = T * K
+    if pairs >= 2 ** 31:
+        refuse(f"T * K ({pairs}) must be below 2^31")
+    device = expert_index.device
+    row_of_pair = torch.empty((T, K), dtype=torch.int32, device=device)
+    H = 0
+    rows = None
+    if hidden is not None:
+        H = hidden.shape[1]
+        rows = torch.empty((pairs, H), dtype=hidden.dtype, device=device)
+    if pairs == 0:
+        return rows, SortedTokens(torch.zeros(E + 1, dtype=torch.int32, device=device), row_of_pair, E)
+    index = expert_index.contiguous()
+    offsets = torch.empty(E + 1, dtype=torch.int32, device=device)
+    size, ws = 0, None
+    if pairs > _ONE_LAUNCH:
+        size = _lib.load_library().b200moe_sort_workspace_bytes(pairs, E)
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+    if H:
+        hidden = unit_rows(hidden)
+        launch(device, "b200moe_sort_tokens", hidden.data_ptr(), _lib.dtype_code(hidden), pitch_of(hidden), index.data_ptr(),
+               index.element_size(), T, K, H, E, offsets.data_ptr(), row_of_pair.data_ptr(), rows.data_ptr(), _lib.ptr(ws), size)
+    else:
+        launch(device, "b200moe_sort_pairs", index.data_ptr(), index.element_size(), T, K, E, offsets.data_ptr(),
+               row_of_pair.data_ptr(), _lib.ptr(ws), size)
+    return rows, SortedTokens(offsets, row_of_pair, E)
 
 
 def moe_sort_plan(expert_index: torch.Tensor, num_experts: int) -> SortedTokens:
     """Sort the pairs of ``expert_index [T, K]`` (int32, uint32 or int64).  Ids outside ``[0, num_experts)``, such as the -1
     of a dropped pair, get no row; equal ids of one token get a row each."""
-    _lib.require_cuda(expert_index)
-    A = _lib.kernel_assert
-    A(expert_index.dim() == 2, "expert_index must be [T, K]")
-    A(expert_index.dtype in (torch.int32, torch.uint32, torch.int64), "expert_index must be int32, uint32 or int64")
-    A(1 <= num_experts <= MAX_EXPERTS, f"num_experts ({num_experts}) must be between 1 and {MAX_EXPERTS}")
-    T, K = expert_index.shape
-    E, pairs = int(num_experts), T * K
-    A(pairs < 2 ** 31, f"T * K ({pairs}) must be below 2^31")
-    device = expert_index.device
-    if pairs == 0:
-        return SortedTokens(torch.zeros(E + 1, dtype=torch.int32, device=device),
-                            torch.empty((T, K), dtype=torch.int32, device=device),
-                            torch.empty(0, dtype=torch.int32, device=device), E)
-    index = expert_index.contiguous()
-    offsets = torch.empty(E + 1, dtype=torch.int32, device=device)
-    row_of_pair = torch.empty((T, K), dtype=torch.int32, device=device)
-    pair_of_row = torch.empty(pairs, dtype=torch.int32, device=device)
-    size = _lib.load_library().b200moe_sort_workspace_bytes(pairs, E)
-    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    launch(device, "b200moe_sort_pairs", index.data_ptr(), index.element_size(), T, K, E, offsets.data_ptr(),
-           row_of_pair.data_ptr(), pair_of_row.data_ptr(), _lib.ptr(ws), size)
-    return SortedTokens(offsets, row_of_pair, pair_of_row, E)
+    return _sort(expert_index, num_experts, None)[1]
 
 
 def _check_plan(plan: SortedTokens) -> Tuple[int, int]:
-    A = _lib.kernel_assert
-    A(isinstance(plan, SortedTokens), "plan must be the SortedTokens of moe_sort_plan or moe_sort_tokens")
-    A(plan.row_of_pair.dim() == 2 and plan.row_of_pair.dtype == torch.int32 and plan.row_of_pair.is_contiguous() and
-      plan.expert_offsets.dtype == torch.int32 and plan.expert_offsets.is_contiguous() and
-      plan.expert_offsets.numel() == plan.num_experts + 1, "plan must be as moe_sort_plan made it")
-    return plan.row_of_pair.shape
+    if not isinstance(plan, SortedTokens):
+        refuse("plan must be the SortedTokens of moe_sort_plan or moe_sort_tokens")
+    row, offsets = plan.row_of_pair, plan.expert_offsets
+    if not (row.dim() == 2 and row.dtype == torch.int32 and row.is_contiguous() and offsets.dtype == torch.int32 and
+            offsets.is_contiguous() and offsets.numel() == plan.num_experts + 1):
+        refuse("plan must be as moe_sort_plan made it")
+    return row.shape
 
 
 def _check_rows(t: torch.Tensor, name: str) -> None:
-    _lib.kernel_assert(t.dim() == 2 and t.dtype in (torch.bfloat16, torch.float32), f"{name} must be 2-D, bfloat16 or float32")
-
-
-def _sort_rows(hidden: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
-    T, K = plan.row_of_pair.shape
-    H = hidden.shape[1]
-    rows = torch.empty((T * K, H), dtype=hidden.dtype, device=hidden.device)
-    if rows.numel():
-        hidden = unit_rows(hidden)
-        launch(hidden.device, "b200moe_sort_rows", hidden.data_ptr(), _lib.dtype_code(hidden), pitch_of(hidden), T, K, H,
-               plan.num_experts, plan.row_of_pair.data_ptr(), plan.expert_offsets.data_ptr(), rows.data_ptr())
-    return rows
+    if t.dim() != 2 or t.dtype not in (torch.bfloat16, torch.float32):
+        refuse(f"{name} must be 2-D, bfloat16 or float32")
 
 
 def _unsort_rows(rows: torch.Tensor, affinities: Optional[torch.Tensor], plan: SortedTokens) -> torch.Tensor:
@@ -91,16 +101,18 @@ def _unsort_rows(rows: torch.Tensor, affinities: Optional[torch.Tensor], plan: S
     return out
 
 
-class _SortRows(torch.autograd.Function):
+class _SortTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, plan):
-        ctx.plan = plan
-        return _sort_rows(hidden, plan)
+    def forward(ctx, hidden, expert_index, num_experts):
+        rows, ctx.plan = _sort(expert_index, num_experts, hidden)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(ctx.plan.expert_offsets, ctx.plan.row_of_pair)
+        return rows, ctx.plan.expert_offsets, ctx.plan.row_of_pair
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_rows):
-        return _unsort_rows(d_rows, None, ctx.plan), None
+    @once
+    def backward(ctx, d_rows, _offsets, _row_of_pair):
+        return (None if d_rows is None else _unsort_rows(d_rows, None, ctx.plan)), None, None
 
 
 class _UnsortRows(torch.autograd.Function):
@@ -112,7 +124,7 @@ class _UnsortRows(torch.autograd.Function):
         return _unsort_rows(rows, affinities, plan)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, d_out):
         rows, affinities = ctx.saved_tensors
         plan = ctx.plan
@@ -146,10 +158,12 @@ def moe_sort_tokens(hidden: torch.Tensor, expert_index: torch.Tensor,
     """
     same_device(hidden, expert_index)
     _check_rows(hidden, "hidden")
-    _lib.kernel_assert(expert_index.dim() == 2 and expert_index.shape[0] == hidden.shape[0],
-                       "expert_index must be [T, K] with hidden's T")
-    plan = moe_sort_plan(expert_index, num_experts)
-    return (_SortRows.apply(hidden, plan) if needs_grad(hidden) else _sort_rows(hidden, plan)), plan
+    if expert_index.dim() != 2 or expert_index.shape[0] != hidden.shape[0]:
+        refuse("expert_index must be [T, K] with hidden's T")
+    if not needs_grad(hidden):
+        return _sort(expert_index, num_experts, hidden)
+    rows, offsets, row_of_pair = _SortTokens.apply(hidden, expert_index, num_experts)
+    return rows, SortedTokens(offsets, row_of_pair, int(num_experts))
 
 
 def moe_unsort_tokens(rows: torch.Tensor, affinities: Optional[torch.Tensor], plan: SortedTokens) -> torch.Tensor:
@@ -160,13 +174,14 @@ def moe_unsort_tokens(rows: torch.Tensor, affinities: Optional[torch.Tensor], pl
     sum.  Products and sums are fp32, in the order of the choices, rounded once; a token without rows comes out zero.
     Differentiable in ``rows`` (rows behind the last expert get zero) and ``affinities`` (zero for a pair without a row).
     """
-    same_device(rows, affinities, plan.row_of_pair)
     T, K = _check_plan(plan)
+    same_device(rows, affinities, plan.row_of_pair, plan.expert_offsets)
     _check_rows(rows, "rows")
-    _lib.kernel_assert(rows.shape[0] == T * K, f"rows must hold T * K ({T * K}) rows, got {rows.shape[0]}")
-    if affinities is not None:
-        _lib.kernel_assert(tuple(affinities.shape) == (T, K) and affinities.dtype in (torch.float32, torch.bfloat16),
-                           f"affinities must be [T, K] = [{T}, {K}], float32 or bfloat16")
+    if rows.shape[0] != T * K:
+        refuse(f"rows must hold T * K ({T * K}) rows, got {rows.shape[0]}")
+    if affinities is not None and (affinities.shape != plan.row_of_pair.shape or
+                                   affinities.dtype not in (torch.float32, torch.bfloat16)):
+        refuse(f"affinities must be [T, K] = [{T}, {K}], float32 or bfloat16")
     if needs_grad(rows, affinities):
         return _UnsortRows.apply(rows, affinities, plan)
     return _unsort_rows(rows, affinities, plan)

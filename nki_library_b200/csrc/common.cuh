@@ -107,14 +107,14 @@ __device__ __forceinline__ void grid_enter(P&... pointers) {
 // plain edges are the cheaper ones (16-token decode step, seven kernels: 274.7 us with plain, 280.7 with programmatic
 // edges), while eagerly the overlap takes the 64-token decode from 261.7 to 255.3 us, the fp8-row one from 139.4 to 131.4.
 template <typename... P, typename... A>
-inline cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, unsigned block, size_t smem, cudaStream_t st,
+inline cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                                      A&&... args) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(block);
+  cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;

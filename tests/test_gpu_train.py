@@ -49,9 +49,9 @@ def test_order(T, K, E, dropped, repeat, dtype):
     if T > 2:
         idx[1, 0], idx[2, 0] = E, 2 ** 31 - 1  # no expert either
     plan = m.moe_sort_plan(idx, E)
-    offsets, row, pair = ref.sorted_rows(idx, E)
+    offsets, row = ref.sorted_rows(idx, E)
     assert torch.equal(plan.expert_offsets.cpu(), offsets)
-    assert torch.equal(plan.row_of_pair.cpu(), row) and torch.equal(plan.pair_of_row.cpu(), pair)
+    assert torch.equal(plan.row_of_pair.cpu(), row)
     assert plan.num_experts == E
 
 
@@ -63,7 +63,7 @@ def test_order_of_unsigned_strided_and_no_ids():
     wide[:, ::2] = idx
     for other in (idx.view(torch.uint32), wide[:, ::2], idx.t().contiguous().t()):
         got = m.moe_sort_plan(other, 16)
-        assert all(torch.equal(a, b) for a, b in zip(got[:3], want[:3]))
+        assert all(torch.equal(a, b) for a, b in zip(got[:2], want[:2]))
     for shape in ((0, 4), (4, 0)):
         rows, plan = m.moe_sort_tokens(torch.ones(shape[0], 8, device="cuda"), idx[:shape[0], :shape[1]], 16)
         assert rows.shape == (0, 8) and plan.expert_offsets.tolist() == [0] * 17
@@ -362,7 +362,7 @@ def test_activation_and_gradient(R, I, act):
 @pytest.mark.parametrize("I", [8, 32, 104, 2048])
 def test_checkpoint_is_exact(I):
     """Codes and scales bit for bit: magnitudes from the smallest to the largest, ties, blocks of zeros, NaN and infinity."""
-    from nki_library_b200.core.moe.moe_train.moe_glu import glu_backward, glu_forward
+    from nki_library_b200.core.moe.moe_train.moe_glu import glu_backward, glu_forward, kept_parts
     R = 96
     gen = _gen(I)
     x = torch.randn((R, 2 * I), device="cuda", generator=gen) * torch.exp2(
@@ -376,7 +376,8 @@ def test_checkpoint_is_exact(I):
     x[14], x[14, 2] = 2.0 ** -133, 3.3e38
     x[15] = 2.0 ** -133
     x = x.bfloat16()
-    _, codes, scales = glu_forward(x, 0, True)
+    _, checkpoint = glu_forward(x, 0, True)
+    codes, scales = kept_parts(checkpoint, R, I)
     e, g, u = _kept_reference(x)
     assert torch.equal(scales.long() - 127, e)
     s = ref.power_of_two(e).repeat_interleave(32, 2)[:, :, :I].reshape(R, 2 * I)
@@ -385,13 +386,14 @@ def test_checkpoint_is_exact(I):
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
     # and what the backward pass makes of it: m from the kept values
     with torch.no_grad():
-        _, again = glu_backward(torch.ones((R, I), device="cuda").bfloat16(), codes, scales, 0, want_m=True)
+        _, again = glu_backward(torch.ones((R, I), device="cuda").bfloat16(), checkpoint, 0, want_m=True)
     a, _ = ref.act_and_slope(g, "SiLU")
     want = a * u
     rows = want.abs().amax(1) < 1e30  # also drops rows with NaN
     assert rows.sum() > 20
-    # exp(-g) is infinite in fp32 below g = -88.72, where act(g) is smaller than 88.72 exp(-88.72) = 2.7e-37: act becomes 0
-    _close(again[rows], want[rows], want[rows].abs(), 1, want[rows].abs() * 2.0 ** -16 + 2.7e-37 * u[rows].abs())
+    # 1 / (1 + exp(-g)) is flushed to zero below 2^-126, for g below -87.33, where act(g) is smaller than 87.34 * 2^-126 =
+    # 1.03e-36
+    _close(again[rows], want[rows], want[rows].abs(), 1, want[rows].abs() * 2.0 ** -16 + 1.03e-36 * u[rows].abs())
     bad = g.isnan() | u.isnan()
     assert torch.equal(again.isnan() & bad, bad)
 
@@ -462,8 +464,8 @@ def test_layer_is_its_operators(T, K, E, H, I, dropped):
     for g, w in zip(grads, want):
         assert torch.equal(g, w)
     with torch.no_grad():
-        _, codes, scales = glu_forward(gate_up, 0, True)
-        _, m_kept = glu_backward(act, codes, scales, 0, want_m=True)
+        _, checkpoint = glu_forward(gate_up, 0, True)
+        _, m_kept = glu_backward(act, checkpoint, 0, want_m=True)
         assert torch.equal(grads[3], weight_grad(m_kept, d_y, w2, plan.expert_offsets))
         assert torch.equal(m.moe_experts_train(*(t.detach() if t.is_floating_point() else t for t in (hidden, aff)), idx,
                                                w1.detach(), w2.detach()), out)

@@ -14,12 +14,14 @@ def _refused(name, *args):
 
 
 @pytest.mark.parametrize("name,args,code,message", [
-    ("b200moe_sort_pairs", (None, 4, 4, 2, 8, P, P, P, None, 0, None), -1, "null pointer"),
-    ("b200moe_sort_pairs", (P, 2, 4, 2, 8, P, P, P, None, 0, None), -1, "4 or 8 bytes"),
-    ("b200moe_sort_pairs", (P, 4, 0, 2, 8, P, P, P, None, 0, None), -1, "T, K > 0"),
-    ("b200moe_sort_pairs", (P, 4, 1 << 30, 4, 8, P, P, P, None, 0, None), -1, "pairs"),
-    ("b200moe_sort_pairs", (P, 4, 4, 2, 1025, P, P, P, None, 0, None), -1, "experts"),
-    ("b200moe_sort_pairs", (P, 4, 4096, 2, 8, P, P, P, None, 0, None), -3, "workspace"),
+    ("b200moe_sort_pairs", (None, 4, 4, 2, 8, P, P, None, 0, None), -1, "null pointer"),
+    ("b200moe_sort_pairs", (P, 2, 4, 2, 8, P, P, None, 0, None), -1, "4 or 8 bytes"),
+    ("b200moe_sort_pairs", (P, 4, 0, 2, 8, P, P, None, 0, None), -1, "T, K > 0"),
+    ("b200moe_sort_pairs", (P, 4, 1 << 30, 4, 8, P, P, None, 0, None), -1, "pairs"),
+    ("b200moe_sort_pairs", (P, 4, 4, 2, 1025, P, P, None, 0, None), -1, "experts"),
+    ("b200moe_sort_pairs", (P, 4, 4096, 2, 8, P, P, None, 0, None), -3, "workspace"),
+    ("b200moe_sort_tokens", (P, 2, 64, P, 4, 4, 2, 64, 8, P, P, P, None, 0, None), -1, "fp32 or bf16"),
+    ("b200moe_sort_tokens", (P, 1, 64, P, 3, 4, 2, 64, 8, P, P, P, None, 0, None), -1, "4 or 8 bytes"),
     ("b200moe_sort_rows", (P, 2, 64, 4, 2, 64, 8, P, P, P, None), -1, "fp32 or bf16"),
     ("b200moe_sort_rows", (P, 1, 64, 4, 2, 0, 8, P, P, P, None), -1, "H > 0"),
     ("b200moe_sort_rows", (P, 1, 64, 4, 2, 64, 0, P, P, P, None), -1, "experts"),
@@ -57,7 +59,7 @@ def test_entry_points_refuse(name, args, code, message):
 def test_cpu_tensors_are_refused():
     import nki_library_b200 as m
     x, idx = torch.zeros(4, 64), torch.zeros(4, 2, dtype=torch.int32)
-    plan = m.SortedTokens(torch.zeros(9, dtype=torch.int32), idx, torch.zeros(8, dtype=torch.int32), 8)
+    plan = m.SortedTokens(torch.zeros(9, dtype=torch.int32), idx, 8)
     w = torch.zeros(8, 64, 64, dtype=torch.bfloat16)
     for call in (lambda: m.moe_sort_plan(idx, 8), lambda: m.moe_sort_tokens(x, idx, 8),
                  lambda: m.moe_unsort_tokens(torch.zeros(8, 64), None, plan),

@@ -6,7 +6,7 @@ import torch
 
 
 def sorted_rows(index, E):
-    """(offsets, row_of_pair, pair_of_row) of ids [T, K], on the CPU."""
+    """(offsets, row_of_pair) of ids [T, K], on the CPU."""
     T, K = index.shape
     flat = index.reshape(-1).long().cpu()
     per_expert = [(flat == e).nonzero()[:, 0] for e in range(E)]
@@ -14,9 +14,7 @@ def sorted_rows(index, E):
     offsets = torch.tensor([0] + [p.numel() for p in per_expert]).cumsum(0)
     row = torch.full((T * K,), -1)
     row[order] = torch.arange(order.numel())
-    pair = torch.full((T * K,), -1)
-    pair[:order.numel()] = order
-    return offsets.int(), row.view(T, K).int(), pair.int()
+    return offsets.int(), row.view(T, K).int()
 
 
 def power_of_two(e):
