@@ -15,12 +15,13 @@
 // and half of the rows per 64 contraction steps, 64 bytes per SM and tensor-pipe clock for a full tile, the smallest feed
 // that two accumulators in TMEM allow.
 //
-// Warps of a persistent CTA (256 threads, weight grad 384):
+// Warps of a persistent CTA (256 threads, weight grad 416):
 //   0, 3   TMA producers of the column and the row operand
 //   1      allocates TMEM; in the even CTA issues the MMAs (M 256, K 16), in the odd one hands out the pair's tiles
-//   2      weight grad: fetches the rows of a contraction that do not fill a step of 16 into a buffer of their own and
-//          clears those behind them, which belong to the next expert (or hold what a caller left behind the last one), so
-//          that they add nothing, whatever they hold
+//   last   weight grad: fetches the rows of a contraction that do not fill a step of 16 into a buffer of their own, where
+//   2      clears those behind them, which belong to the next expert (or hold what a caller left behind the last one), so
+//          that they add nothing, whatever they hold.  (One warp for both waits out each copy before it asks for the next:
+//          64 experts of 2048 x 2048, 125 rows each, 152 us, 131 so.)
 //   4..    epilogue: groups of four warps take chunks of 32 output rows in turn.  An accumulator lane is an output column, so
 //          the 32 values a warp holds of a row are 64 contiguous bytes and go straight out.  Turning a chunk around in
 //          shared memory for longer stores costs the tensor pipe operand bandwidth, which the ring's copies and the MMAs
@@ -80,7 +81,7 @@ template <bool WGRAD>
 struct Config {
   static constexpr int kGroups = WGRAD ? 2 : 1;  // of epilogue warps
   static constexpr int kTails = WGRAD ? 2 : 0;
-  static constexpr int kThreads = 128 + kGroups * 128;
+  static constexpr int kThreads = 128 + kGroups * 128 + (WGRAD ? 32 : 0);
   static constexpr int kOffTail = kStages * kStage;
   static constexpr int kOffBar = kOffTail + kTails * kTail;
   static constexpr int kOffSched = kOffBar + 512;
@@ -457,15 +458,36 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
   } else if (WGRAD && warp == 2) {
     if constexpr (WGRAD) {
     // ------------------------------------------------------------ ragged ends
+    int ends = 0;
+    for (int tile = walk.next(); tile >= 0; tile = walk.next()) {
+      const int rest = decode_tile<WGRAD>(p, s, tile).k & 15;
+      if (rest == 0) continue;
+      const int b = ends % C::kTails;
+      uint8_t* base = smem + C::kOffTail + b * kTail;
+      if (!mbar_wait(&tail_full[b], ends / C::kTails & 1, abort_flag, p.status, 45)) break;
+      // 32 lanes clear 512 bytes: a row of all four boxes
+      for (int r = rest; r < 16; ++r)
+        *reinterpret_cast<uint4*>(base + (lane >> 3) * 2048 + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_leader(&tail_ready[b]);
+      ++ends;
+    }
+    }
+  } else if (WGRAD && warp == kThreads / 32 - 1) {
+    if constexpr (WGRAD) {
+    // ------------------------------------------------------------ producer of ragged ends
     const bool leader = elect_one();
     int ends = 0;
     for (int tile = walk.next(); tile >= 0; tile = walk.next()) {
       const Tile t = decode_tile<WGRAD>(p, s, tile);
-      const int rest = t.k & 15;
-      if (rest == 0) continue;
+      if ((t.k & 15) == 0) continue;
       const int b = ends % C::kTails;
       uint8_t* base = smem + C::kOffTail + b * kTail;
-      if (!mbar_wait(&tail_empty[b], (ends / C::kTails & 1) ^ 1u, abort_flag, p.status, 45)) break;
+      if (!mbar_wait(&tail_empty[b], (ends / C::kTails & 1) ^ 1u, abort_flag, p.status, 49)) {
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+        break;
+      }
       if (leader) {
         const int c = t.c0 + rank * 128, r = t.row0 + rank * 128, k = t.k0 + (t.k & ~15);
         mbar_expect_tx(&tail_full[b], kTail);
@@ -474,17 +496,6 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
         tma_load_2d(base + 4096, &row_map.size[2], r, k, &tail_full[b]);
         tma_load_2d(base + 6144, &row_map.size[2], r + 64, k, &tail_full[b]);
       }
-      __syncwarp();
-      if (!mbar_wait(&tail_full[b], ends / C::kTails & 1, abort_flag, p.status, 45)) {
-        for (int i = 0; i < 2000; ++i) __nanosleep(1000);
-        break;
-      }
-      // 32 lanes clear 512 bytes: a row of all four boxes
-      for (int r = rest; r < 16; ++r)
-        *reinterpret_cast<uint4*>(base + (lane >> 3) * 2048 + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive_leader(&tail_ready[b]);
       ++ends;
     }
     }
