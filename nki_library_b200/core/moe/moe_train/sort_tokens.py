@@ -86,8 +86,8 @@ def _check_rows(t: torch.Tensor, name: str) -> None:
         refuse(f"{name} must be 2-D, bfloat16 or float32")
 
 
-def _unsort_rows(rows: torch.Tensor, affinities: Optional[torch.Tensor], plan: SortedTokens) -> torch.Tensor:
-    T, K = plan.row_of_pair.shape
+def _unsort_rows(rows: torch.Tensor, affinities: Optional[torch.Tensor], row_of_pair: torch.Tensor) -> torch.Tensor:
+    T, K = row_of_pair.shape
     H = rows.shape[1]
     if T * K * H == 0:
         return torch.zeros((T, H), dtype=rows.dtype, device=rows.device)
@@ -96,7 +96,7 @@ def _unsort_rows(rows: torch.Tensor, affinities: Optional[torch.Tensor], plan: S
     if affinities is not None:
         affinities = affinities.contiguous()
     launch(rows.device, "b200moe_unsort_rows", rows.data_ptr(), _lib.dtype_code(rows), pitch_of(rows), T, K, H,
-           plan.row_of_pair.data_ptr(), _lib.ptr(affinities), _lib.F32 if affinities is None else _lib.dtype_code(affinities),
+           row_of_pair.data_ptr(), _lib.ptr(affinities), _lib.F32 if affinities is None else _lib.dtype_code(affinities),
            out.data_ptr())
     return out
 
@@ -104,37 +104,38 @@ def _unsort_rows(rows: torch.Tensor, affinities: Optional[torch.Tensor], plan: S
 class _SortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, expert_index, num_experts):
-        rows, ctx.plan = _sort(expert_index, num_experts, hidden)
+        rows, plan = _sort(expert_index, num_experts, hidden)
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(ctx.plan.expert_offsets, ctx.plan.row_of_pair)
-        return rows, ctx.plan.expert_offsets, ctx.plan.row_of_pair
+        ctx.mark_non_differentiable(plan.expert_offsets, plan.row_of_pair)
+        ctx.save_for_backward(plan.row_of_pair)
+        return rows, plan.expert_offsets, plan.row_of_pair
 
     @staticmethod
     @once
     def backward(ctx, d_rows, _offsets, _row_of_pair):
-        return (None if d_rows is None else _unsort_rows(d_rows, None, ctx.plan)), None, None
+        row_of_pair, = ctx.saved_tensors
+        return (None if d_rows is None else _unsort_rows(d_rows, None, row_of_pair)), None, None
 
 
 class _UnsortRows(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, affinities, plan):
+    def forward(ctx, rows, affinities, row_of_pair, expert_offsets):
         # the rows are needed for the affinities' gradient only
-        ctx.save_for_backward(rows if affinities is not None and affinities.requires_grad else None, affinities)
-        ctx.plan = plan
-        return _unsort_rows(rows, affinities, plan)
+        ctx.save_for_backward(rows if affinities is not None and affinities.requires_grad else None, affinities, row_of_pair,
+                              expert_offsets)
+        return _unsort_rows(rows, affinities, row_of_pair)
 
     @staticmethod
     @once
     def backward(ctx, d_out):
-        rows, affinities = ctx.saved_tensors
-        plan = ctx.plan
-        T, K = plan.row_of_pair.shape
+        rows, affinities, row_of_pair, offsets = ctx.saved_tensors
+        T, K = row_of_pair.shape
         H = d_out.shape[1]
         want_rows, want_aff = ctx.needs_input_grad[:2]
         d_rows = torch.empty((T * K, H), dtype=d_out.dtype, device=d_out.device) if want_rows else None
         d_aff = torch.empty((T, K), dtype=affinities.dtype, device=d_out.device) if want_aff else None
         if T * K * H == 0:
-            return d_rows, None if d_aff is None else d_aff.zero_(), None
+            return d_rows, None if d_aff is None else d_aff.zero_(), None, None
         d_out = unit_rows(d_out)
         if want_aff:
             rows = unit_rows(rows)
@@ -142,9 +143,9 @@ class _UnsortRows(torch.autograd.Function):
             affinities = affinities.contiguous()
         launch(d_out.device, "b200moe_unsort_rows_backward", d_out.data_ptr(), pitch_of(d_out),
                rows.data_ptr() if want_aff else None, pitch_of(rows) if want_aff else H, _lib.dtype_code(d_out), T, K, H,
-               plan.num_experts, plan.row_of_pair.data_ptr(), plan.expert_offsets.data_ptr(), _lib.ptr(affinities),
+               offsets.numel() - 1, row_of_pair.data_ptr(), offsets.data_ptr(), _lib.ptr(affinities),
                _lib.F32 if affinities is None else _lib.dtype_code(affinities), _lib.ptr(d_rows), _lib.ptr(d_aff))
-        return d_rows, d_aff, None
+        return d_rows, d_aff, None, None
 
 
 def moe_sort_tokens(hidden: torch.Tensor, expert_index: torch.Tensor,
@@ -183,5 +184,5 @@ def moe_unsort_tokens(rows: torch.Tensor, affinities: Optional[torch.Tensor], pl
                                    affinities.dtype not in (torch.float32, torch.bfloat16)):
         refuse(f"affinities must be [T, K] = [{T}, {K}], float32 or bfloat16")
     if needs_grad(rows, affinities):
-        return _UnsortRows.apply(rows, affinities, plan)
-    return _unsort_rows(rows, affinities, plan)
+        return _UnsortRows.apply(rows, affinities, plan.row_of_pair, plan.expert_offsets)
+    return _unsort_rows(rows, affinities, plan.row_of_pair)

@@ -280,6 +280,11 @@ EncodeTiledFn get_encode_fn() {
         qres == cudaDriverEntryPointSuccess)
       fn = reinterpret_cast<EncodeTiledFn>(ptr);
   }
+  // The function wants a current context, which a host thread has only once it has set its device: not one that a framework
+  // has just started for a backward pass.
+  thread_local bool bound = false;
+  int dev = 0;
+  if (!bound && cudaGetDevice(&dev) == cudaSuccess) bound = cudaSetDevice(dev) == cudaSuccess;
   return fn;
 }
 

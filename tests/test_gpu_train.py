@@ -255,7 +255,8 @@ def test_products_of_other_layouts_and_orders():
     strided[:, :, 1, 4:164] = w
     padded = torch.zeros((3, 100, 176), dtype=torch.bfloat16, device="cuda")
     padded[:, :96, 8:168] = w
-    for weight in (strided[:, :, 1, 4:164], padded[:, :96, 8:168], w.permute(1, 2, 0).contiguous().permute(2, 0, 1)):
+    for weight in (strided[:, :, 1, 4:164], padded[:, :96, 8:168], w.permute(1, 2, 0).contiguous().permute(2, 0, 1),
+                   w.transpose(0, 1).contiguous().transpose(0, 1), w.permute(2, 0, 1).contiguous().permute(1, 2, 0)):
         leaf = weight.detach().requires_grad_()
         got = m.expert_linear(x, leaf, offsets)
         assert torch.equal(got, want)
@@ -528,6 +529,37 @@ def test_runs_repeat_bit_for_bit_and_on_other_streams():
     torch.cuda.synchronize()
     for got in results:
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_first_call_of_a_thread():
+    """A host thread that has made no CUDA call yet, such as the one a backward pass gets, has no context of its own."""
+    import threading
+
+    import nki_library_b200 as m
+    offsets, x, w, _ = _product_case([40, 24], 64, 128, 0, 1)
+    want = m.expert_linear(x, w, offsets)
+    del want
+    got = []
+    worker = threading.Thread(target=lambda: got.append(m.expert_linear(x, w, offsets)))
+    worker.start()
+    worker.join()
+    assert len(got) == 1 and torch.equal(got[0], m.expert_linear(x, w, offsets))
+
+
+def test_second_derivatives_are_refused():
+    """The passes are recorded as they are called, not differentiated again."""
+    import nki_library_b200 as m
+    idx, leaves, d = _layer(3)
+    leaves = [t.requires_grad_() for t in leaves]
+    out = m.moe_experts_train(leaves[0], leaves[1], idx, leaves[2], leaves[3])
+    first = torch.autograd.grad(out, leaves, d, create_graph=True)
+    plain = torch.autograd.grad(m.moe_experts_train(leaves[0], leaves[1], idx, leaves[2], leaves[3]), leaves, d)
+    assert all(torch.equal(a, b) for a, b in zip(first, plain))
+    d.requires_grad_()
+    out = m.moe_experts_train(leaves[0], leaves[1], idx, leaves[2], leaves[3])
+    first = torch.autograd.grad(out, leaves, d, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        first[0].float().sum().backward()
 
 
 def test_captured_step_replays_on_new_inputs():
