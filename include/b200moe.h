@@ -423,14 +423,18 @@ int b200moe_unsort_rows_backward(const void* d_out, int64_t d_pitch, const void*
 /* Every expert's rows times its matrix, bf16 with fp32 accumulation.  weight: E matrices [D0, D1] with D1 contiguous
  * (pitches in elements).  contract_last 0: rows [R, D0] -> out [R, D1]; 1: rows [R, D1] -> out [R, D0].  Rows of no expert
  * come out zero.  D0 and D1 are multiples of 8; rows and matrices start on 16-byte boundaries.  status: device
- * int32[2], the first as for the grouped contractions (codes 41 to 49), the second scratch. */
+ * int32[2], the first as for the grouped contractions (codes 41 to 49), the second scratch.  workspace: where few tiles
+ * have long contractions these are cut into parts, whose fp32 sums it holds (16-byte aligned; often 0 bytes). */
+size_t b200moe_expert_product_workspace_bytes(int contract_last, int R, int E, int D0, int D1);
 int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch, const void* weight_bf16, int64_t w_pitch,
                            int64_t w_expert_pitch, int contract_last, const int32_t* expert_offsets, int R, int E, int D0,
-                           int D1, void* out_bf16, int32_t* status, b200moe_stream_t stream);
+                           int D1, void* out_bf16, void* workspace, size_t workspace_bytes, int32_t* status,
+                           b200moe_stream_t stream);
 /* out[e] [M, N] = sum over the expert's rows r of a[r, :]^T b[r, :]; zero for an expert without rows. */
+size_t b200moe_expert_weight_grad_workspace_bytes(int R, int E, int M, int N);
 int b200moe_expert_weight_grad(const void* a_bf16, int64_t a_pitch, const void* b_bf16, int64_t b_pitch,
-                               const int32_t* expert_offsets, int R, int E, int M, int N, void* out_bf16, int32_t* status,
-                               b200moe_stream_t stream);
+                               const int32_t* expert_offsets, int R, int E, int M, int N, void* out_bf16, void* workspace,
+                               size_t workspace_bytes, int32_t* status, b200moe_stream_t stream);
 /* m [R, I] = act(gate) * up of gate_up [R, 2 I] (gate first), I a multiple of 8.  codes [R, 2 I] e4m3 and scales
  * [R, 2, ceil(I / 32)] UE8M0 (both NULL: not kept): v is kept as e4m3(v / s), s the smallest power of two of at least 2^-127
  * for which no finite value of the 32 columns exceeds 448 s; a value that is not finite is kept as NaN. */

@@ -118,10 +118,12 @@ SIGNATURES = {
                                     c_void_p]),
     "b200moe_unsort_rows_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int,
                                              c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "b200moe_expert_product_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "b200moe_expert_product": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int, c_int,
-                                       c_int, c_void_p, c_void_p, c_void_p]),
+                                       c_int, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "b200moe_expert_weight_grad_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "b200moe_expert_weight_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int,
-                                           c_void_p, c_void_p, c_void_p]),
+                                           c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "b200moe_glu": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "b200moe_glu_backward": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p,
                                      c_void_p]),

@@ -2,7 +2,7 @@
 
 from __future__ import annotations
 
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -30,6 +30,13 @@ def _stored(weight: torch.Tensor) -> Tuple[torch.Tensor, bool]:
     return weight.clone(memory_format=torch.contiguous_format), False
 
 
+_LONG = 49 * 64  # contractions below this length are never cut into parts, and need no workspace
+
+
+def _workspace(size: int, device: torch.device) -> Tuple[Optional[torch.Tensor], int]:
+    return (torch.empty(size, dtype=torch.uint8, device=device), size) if size else (None, 0)
+
+
 def product(rows: torch.Tensor, weight: torch.Tensor, expert_offsets: torch.Tensor, transpose: bool = False,
             check_status: bool = False) -> torch.Tensor:
     """``rows[r] @ weight[e]``, with ``transpose`` ``rows[r] @ weight[e].T``."""
@@ -42,10 +49,14 @@ def product(rows: torch.Tensor, weight: torch.Tensor, expert_offsets: torch.Tens
         return out
     rows = tile_rows(rows)
     w_pitch = stored.stride(1)
+    ws, ws_bytes = None, 0
+    if rows.shape[1] >= _LONG:
+        ws, ws_bytes = _workspace(_lib.load_library().b200moe_expert_product_workspace_bytes(int(contract_last), R, E, D0, D1),
+                                  rows.device)
     status = torch.empty(2, dtype=torch.int32, device=rows.device)
     launch(rows.device, "b200moe_expert_product", rows.data_ptr(), pitch_of(rows), stored.data_ptr(), w_pitch,
            stored.stride(0) if E > 1 else D0 * w_pitch, int(contract_last), expert_offsets.data_ptr(), R, E, D0, D1,
-           out.data_ptr(), status.data_ptr())
+           out.data_ptr(), _lib.ptr(ws), ws_bytes, status.data_ptr())
     if check_status:
         _lib.kernel_assert(int(status[0].item()) == 0, f"device-side wait expired in expert_linear (status {int(status[0].item())})")
     return out
@@ -63,8 +74,11 @@ def weight_grad(rows: torch.Tensor, d_out: torch.Tensor, weight: torch.Tensor, e
         out = torch.empty((E, M, W), dtype=torch.bfloat16, device=weight.device)
         a, b = tile_rows(a), tile_rows(b)
         status = torch.empty(2, dtype=torch.int32, device=weight.device)
+        R, ws, ws_bytes = rows.shape[0], None, 0
+        if R >= _LONG * E:
+            ws, ws_bytes = _workspace(_lib.load_library().b200moe_expert_weight_grad_workspace_bytes(R, E, M, W), weight.device)
         launch(weight.device, "b200moe_expert_weight_grad", a.data_ptr(), pitch_of(a), b.data_ptr(), pitch_of(b),
-               expert_offsets.data_ptr(), rows.shape[0], E, M, W, out.data_ptr(), status.data_ptr())
+               expert_offsets.data_ptr(), R, E, M, W, out.data_ptr(), _lib.ptr(ws), ws_bytes, status.data_ptr())
     return out.transpose(1, 2) if turned else out
 
 

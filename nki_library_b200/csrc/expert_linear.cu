@@ -29,6 +29,8 @@
 // Every wait is bounded; on expiry a code goes to `status`, no more work is issued and the kernel tears down.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "tcgen05_ptx.cuh"
 
@@ -64,6 +66,9 @@ struct Params {
   int row_tiles, col_tiles;  // product: row_tiles unused
   Divisor per_matrix, per_group;  // tiles of a matrix (weight grad) and of kGroup row tiles
   __nv_bfloat16* out;
+  int parts;         // the contraction is cut into this many; above 1, part i's sums go to partial[i]
+  float* partial;    // [parts][output rows][cols]
+  int64_t out_rows;  // of all experts
   int32_t* status;
   int32_t* taken;  // tiles handed out beyond every pair's first; NULL: pair u walks tiles u, u + pairs, ...
   int queue;       // ... and how many of them a pair holds at most
@@ -77,9 +82,12 @@ struct Sched {
   int queue[kQueue];
 };
 
-template <bool WGRAD>
+// Epilogue groups of four warps: one for a product, whose stores pass while the next tile's contraction runs, two where that is
+// as short as the stores (SHORT; 9216 rows on 6 experts of K x 13376, one group / two: K 64 87 / 73 us, 256 92 / 81; of 512 x 8192
+// 69 / 70, 4096 x 4096 212 / 214) and for the weight grad.
+template <bool WGRAD, bool SHORT>
 struct Config {
-  static constexpr int kGroups = WGRAD ? 2 : 1;  // of epilogue warps
+  static constexpr int kGroups = WGRAD || SHORT ? 2 : 1;
   static constexpr int kTails = WGRAD ? 2 : 0;
   static constexpr int kThreads = 128 + kGroups * 128 + (WGRAD ? 32 : 0);
   static constexpr int kOffTail = kStages * kStage;
@@ -131,7 +139,8 @@ struct Tile {
   int expert;
   int row0, rows;  // output rows: of the row matrix (product), of the expert's matrix (weight grad)
   int c0;          // first output column
-  int k0, k;       // weight grad: the contraction's rows
+  int k0, k;       // the contraction's range (weight grad: of rows)
+  int part;
   // Steps of 16 that the ring brings (a weight grad's ragged end comes through its own buffer), and slabs of four.
   template <bool WGRAD>
   __device__ __forceinline__ int steps() const { return WGRAD ? k >> 4 : (k + 15) >> 4; }
@@ -159,6 +168,12 @@ template <bool WGRAD>
 __device__ __forceinline__ Tile decode_tile(const Params& p, const Sched& s, int tile) {
   Tile t;
   int rt, ct;
+  t.part = 0;
+  if (p.parts > 1) {
+    const int whole = WGRAD ? p.E * p.row_tiles * p.col_tiles : s.tiles[p.E];
+    t.part = tile / whole;
+    tile -= t.part * whole;
+  }
   if constexpr (WGRAD) {
     t.expert = p.per_matrix.quotient(tile);
     grouped_order(p, tile - t.expert * p.row_tiles * p.col_tiles, p.row_tiles, rt, ct);
@@ -184,6 +199,13 @@ __device__ __forceinline__ Tile decode_tile(const Params& p, const Sched& s, int
     t.k = p.k;
   }
   t.c0 = ct * 256;
+  if (p.parts > 1) {  // whole slabs to every part, what is left of the last one to the last part
+    const int64_t slabs = (t.k + 63) >> 6;
+    const int from = static_cast<int>(slabs * t.part / p.parts) * 64;
+    const int to = min(static_cast<int>(slabs * (t.part + 1) / p.parts) * 64, t.k);
+    t.k0 += from;
+    t.k = to - from;
+  }
   return t;
 }
 
@@ -225,10 +247,10 @@ struct Walk {
 struct RowMaps { CUtensorMap size[4]; };
 
 // COL_MN: the column operand is MN-major (always so for the weight grad, whose row operand is too).
-template <bool WGRAD, bool COL_MN>
-__global__ void __launch_bounds__(Config<WGRAD>::kThreads, 1) __cluster_dims__(2, 1, 1)
+template <bool WGRAD, bool COL_MN, bool SHORT>
+__global__ void __launch_bounds__(Config<WGRAD, SHORT>::kThreads, 1) __cluster_dims__(2, 1, 1)
 expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_constant__ RowMaps row_map, const Params p) {
-  using C = Config<WGRAD>;
+  using C = Config<WGRAD, SHORT>;
   constexpr int kGroups = C::kGroups, kThreads = C::kThreads;
   constexpr uint32_t kTmemCols = 512;
   constexpr uint32_t kIdesc = make_idesc_bf16(256, 0) | (COL_MN ? 1u << 15 : 0u) | (WGRAD ? 1u << 16 : 0u);  // N per tile
@@ -317,7 +339,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
   cluster_sync_all();  // the peer's barriers exist before anything signals them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr;
-  const int total = WGRAD ? p.E * p.row_tiles * p.col_tiles : s.tiles[p.E];
+  const int total = (WGRAD ? p.E * p.row_tiles * p.col_tiles : s.tiles[p.E]) * p.parts;
   Walk<!WGRAD> walk{p, s, queue_full, queue_empty, abort_flag, unit, n_units, total, 0};
 
   if (warp == 0) {
@@ -340,10 +362,10 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
             tma2_load_2d(dst, &col_map, c, t.k0 + kb * 64, &full[stage]);
             tma2_load_2d(dst + 8192, &col_map, c + 64, t.k0 + kb * 64, &full[stage]);
           } else if constexpr (COL_MN) {
-            tma2_load_3d(dst, &col_map, c, kb * 64, t.expert, &full[stage]);
-            tma2_load_3d(dst + 8192, &col_map, c + 64, kb * 64, t.expert, &full[stage]);
+            tma2_load_3d(dst, &col_map, c, t.k0 + kb * 64, t.expert, &full[stage]);
+            tma2_load_3d(dst + 8192, &col_map, c + 64, t.k0 + kb * 64, t.expert, &full[stage]);
           } else {
-            tma2_load_3d(dst, &col_map, kb * 64, c, t.expert, &full[stage]);
+            tma2_load_3d(dst, &col_map, t.k0 + kb * 64, c, t.expert, &full[stage]);
           }
         }
         if (++stage == kStages) { stage = 0; phase ^= 1u; }
@@ -372,11 +394,12 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
             tma2_load_2d(dst, &row_map.size[0], r, t.k0 + kb * 64, &full[stage]);
             tma2_load_2d(dst + 8192, &row_map.size[0], r + 64, t.k0 + kb * 64, &full[stage]);
           } else {
+            const int k = t.k0 + kb * 64;
             int at = 0;
-            if (half & 128) { tma2_load_2d(dst, &row_map.size[0], kb * 64, r, &full[stage]); at = 128; }
-            if (half & 64) { tma2_load_2d(dst + at * 128, &row_map.size[1], kb * 64, r + at, &full[stage]); at += 64; }
-            if (half & 32) { tma2_load_2d(dst + at * 128, &row_map.size[2], kb * 64, r + at, &full[stage]); at += 32; }
-            if (half & 16) tma2_load_2d(dst + at * 128, &row_map.size[3], kb * 64, r + at, &full[stage]);
+            if (half & 128) { tma2_load_2d(dst, &row_map.size[0], k, r, &full[stage]); at = 128; }
+            if (half & 64) { tma2_load_2d(dst + at * 128, &row_map.size[1], k, r + at, &full[stage]); at += 64; }
+            if (half & 32) { tma2_load_2d(dst + at * 128, &row_map.size[2], k, r + at, &full[stage]); at += 32; }
+            if (half & 16) tma2_load_2d(dst + at * 128, &row_map.size[3], k, r + at, &full[stage]);
           }
         }
         if (++stage == kStages) { stage = 0; phase ^= 1u; }
@@ -503,7 +526,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3, group = (warp - 4) >> 2;
     int it = 0;
-    if constexpr (!WGRAD) {
+    if (!WGRAD && p.parts == 1) {
       // rows of no expert
       const int lo = s.first[0], hi = s.first[p.E], none = lo + p.R - hi;
       for (int i = blockIdx.x * 4 * kGroups + warp - 4; i < none; i += gridDim.x * 4 * kGroups) {
@@ -514,10 +537,16 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
     for (int tile = walk.next(); tile >= 0; tile = walk.next()) {
       const Tile t = decode_tile<WGRAD>(p, s, tile);
       const int64_t row0 = (WGRAD ? static_cast<int64_t>(t.expert) * p.rows : 0) + t.row0;
-      if (WGRAD && t.k == 0) {  // an expert without rows: zeros, eight columns per thread
+      if (WGRAD && t.k == 0) {  // an expert without rows, or a part without: zeros, eight columns per thread
         const int c = t.c0 + rank * 128 + (lane & 15) * 8;
-        for (int r = (warp - 4) * 2 + (lane >> 4); r < t.rows && c < p.cols; r += 8 * kGroups)
-          *reinterpret_cast<uint4*>(p.out + (row0 + r) * p.cols + c) = make_uint4(0, 0, 0, 0);
+        for (int r = (warp - 4) * 2 + (lane >> 4); r < t.rows && c < p.cols; r += 8 * kGroups) {
+          if (p.parts == 1) {
+            *reinterpret_cast<uint4*>(p.out + (row0 + r) * p.cols + c) = make_uint4(0, 0, 0, 0);
+          } else {
+            uint4* o = reinterpret_cast<uint4*>(p.partial + (t.part * p.out_rows + row0 + r) * p.cols + c);
+            o[0] = o[1] = make_uint4(0, 0, 0, 0);
+          }
+        }
         continue;
       }
       const int col = t.c0 + rank * 128 + q * 32 + lane;
@@ -541,7 +570,12 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
           if (lane == 0) mbar_arrive_leader_relaxed(&tmem_empty[acc]);
         }
         const int rows = min(32, t.rows - c * 32);
-        if (col < p.cols) {
+        if (col < p.cols && p.parts > 1) {
+          float* o = p.partial + (t.part * p.out_rows + row0 + c * 32) * p.cols + col;
+#pragma unroll
+          for (int j = 0; j < 32; ++j, o += p.cols)
+            if (j < rows) *o = __uint_as_float(v[j]);
+        } else if (col < p.cols) {
           __nv_bfloat16* o = out;
           if (rows == 32) {
 #pragma unroll
@@ -567,6 +601,60 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
   }
 }
 
+// out = the parts' sums, added up in their order.  Eight columns per thread; rows of no expert (a product's: `offsets`) are zero.
+__global__ void __launch_bounds__(256) join_parts_kernel(const float* partial, int parts, int64_t rows, int cols, const int32_t* offsets,
+                                                         int E, __nv_bfloat16* out) {
+  __shared__ int s_last;
+  grid_enter(partial, offsets);
+  int64_t lo = 0, hi = rows;
+  if (offsets != nullptr) {  // the experts' rows go from the first offset to the largest one
+    if (threadIdx.x == 0) s_last = 0;
+    __syncthreads();
+    int last = 0;
+    for (int e = threadIdx.x; e <= E; e += 256) last = max(last, offsets[e]);
+    atomicMax(&s_last, last);
+    __syncthreads();
+    lo = min(max(static_cast<int64_t>(offsets[0]), int64_t{0}), rows);
+    hi = min(static_cast<int64_t>(s_last), rows);
+  }
+  const int64_t pieces = rows * (cols >> 3), stride = rows * cols;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < pieces; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / (cols >> 3);
+    uint4 result = make_uint4(0, 0, 0, 0);
+    if (row >= lo && row < hi) {
+      float sum[8] = {};
+#pragma unroll 4
+      for (int part = 0; part < parts; ++part) {
+        const float4* f = reinterpret_cast<const float4*>(partial + part * stride + i * 8);
+        const float4 a = __ldcg(f), b = __ldcg(f + 1);
+        sum[0] += a.x; sum[1] += a.y; sum[2] += a.z; sum[3] += a.w;
+        sum[4] += b.x; sum[5] += b.y; sum[6] += b.z; sum[7] += b.w;
+      }
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(sum[2 * j], sum[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+      result = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    *reinterpret_cast<uint4*>(out + i * 8) = result;
+  }
+}
+
+// Parts to cut a contraction of `slabs` into where its `tiles` leave more than half of the CTA pairs idle: as many as there are
+// pairs for, of eight slabs at least.  The join costs a launch, so each part has to save 48 slabs of about 0.25 us.  Without /
+// with: 64 rows on 2 experts of 28672 x 512 105 / 26 us, 454 on 9 of 21304 x 560 85 / 55, weight gradient of 65536 rows on 2 of
+// 256 x 512 152 / 36; 64 rows on one of 4096 x 4096, two parts, 22.0 / 24.6, which is why the bound is there.
+int split_parts(int64_t tiles, int64_t slabs) {
+  const int64_t units = sm_count() / 2;
+  if (tiles * 2 > units) return 1;
+  const int64_t parts = units / tiles < slabs / 8 ? units / tiles : slabs / 8;
+  return parts > 1 && slabs - slabs / parts >= 48 ? static_cast<int>(parts) : 1;
+}
+int64_t product_tiles(int R, int E, int n) { return (ceil_div64(R, 256) + (E < R ? E : R)) * ceil_div64(n, 256); }
+int64_t weight_grad_tiles(int E, int M, int N) { return E * ceil_div64(M, 256) * ceil_div64(N, 256); }
+
 // bf16 matrix (or `batch` of them) with `cols` contiguous; boxes of 64 columns (128 bytes) x box_rows.
 int make_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t pitch, int64_t batch,
              int64_t batch_pitch, int box_rows) {
@@ -584,14 +672,22 @@ int make_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int
   return B200MOE_OK;
 }
 
-template <bool WGRAD, bool COL_MN>
+template <bool WGRAD, bool COL_MN, bool SHORT>
 int launch(const CUtensorMap& cols, const RowMaps& rows, const Params& p, int64_t tiles, cudaStream_t st) {
-  auto kern = expert_linear_kernel<WGRAD, COL_MN>;
-  B200MOE_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), Config<WGRAD>::kSmem));
-  const int64_t units = sm_count() / 2;
-  B200MOE_CUDA_OK(launch_overlapped(kern, dim3(static_cast<unsigned>(2 * (tiles < units ? tiles : units))), Config<WGRAD>::kThreads,
-                                    Config<WGRAD>::kSmem, st, cols, rows, p));
+  auto kern = expert_linear_kernel<WGRAD, COL_MN, SHORT>;
+  using C = Config<WGRAD, SHORT>;
+  B200MOE_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmem));
+  const int64_t units = sm_count() / 2, work = tiles * p.parts;
+  B200MOE_CUDA_OK(launch_overlapped(kern, dim3(static_cast<unsigned>(2 * (work < units ? work : units))), C::kThreads, C::kSmem, st,
+                                    cols, rows, p));
   B200MOE_LAUNCH_OK("expert_linear_kernel");
+  if (p.parts > 1) {
+    const int64_t pieces = p.out_rows * (p.cols / 8), ctas = ceil_div64(pieces, 256), most = static_cast<int64_t>(sm_count()) * 8;
+    B200MOE_CUDA_OK(launch_overlapped(join_parts_kernel, dim3(static_cast<unsigned>(ctas < most ? ctas : most)), 256, 0, st,
+                                      static_cast<const float*>(p.partial), p.parts, p.out_rows, p.cols,
+                                      WGRAD ? static_cast<const int32_t*>(nullptr) : p.offsets, p.E, p.out));
+    B200MOE_LAUNCH_OK("join_parts_kernel");
+  }
   return B200MOE_OK;
 }
 
@@ -604,9 +700,23 @@ bool rows_ok(const void* p, int64_t pitch, int cols) {
 
 using namespace b200moe;
 
+extern "C" size_t b200moe_expert_product_workspace_bytes(int contract_last, int R, int E, int D0, int D1) {
+  if (R <= 0 || E <= 0 || D0 <= 0 || D1 <= 0) return 0;
+  const int k = contract_last ? D1 : D0, n = contract_last ? D0 : D1;
+  const int parts = split_parts(product_tiles(R, E, n), ceil_div64(k, 64));
+  return parts > 1 ? static_cast<size_t>(parts) * R * n * sizeof(float) : 0;
+}
+
+extern "C" size_t b200moe_expert_weight_grad_workspace_bytes(int R, int E, int M, int N) {
+  if (R <= 0 || E <= 0 || M <= 0 || N <= 0) return 0;
+  const int parts = split_parts(weight_grad_tiles(E, M, N), R / (static_cast<int64_t>(E) * 64));
+  return parts > 1 ? static_cast<size_t>(parts) * E * M * N * sizeof(float) : 0;
+}
+
 extern "C" int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch, const void* weight_bf16, int64_t w_pitch,
                                       int64_t w_expert_pitch, int contract_last, const int32_t* expert_offsets, int R, int E,
-                                      int D0, int D1, void* out_bf16, int32_t* status, b200moe_stream_t stream) {
+                                      int D0, int D1, void* out_bf16, void* workspace, size_t workspace_bytes, int32_t* status,
+                                      b200moe_stream_t stream) {
   B200MOE_REQUIRE(rows_bf16 && weight_bf16 && expert_offsets && out_bf16 && status, B200MOE_ERR_INVALID,
                   "expert_product: null pointer argument");
   B200MOE_REQUIRE(R > 0 && E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID,
@@ -630,7 +740,13 @@ extern "C" int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch,
   p.per_matrix = p.per_group = make_divisor(static_cast<uint32_t>(kGroup * p.col_tiles));
   p.out = static_cast<__nv_bfloat16*>(out_bf16);
   p.status = status;
-  const int64_t most_tiles = (ceil_div64(R, 256) + (E < R ? E : R)) * p.col_tiles;
+  const int64_t most_tiles = product_tiles(R, E, n);
+  p.parts = split_parts(most_tiles, ceil_div64(k, 64));
+  p.partial = static_cast<float*>(workspace);
+  p.out_rows = R;
+  B200MOE_REQUIRE(p.parts == 1 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
+                                   workspace_bytes >= b200moe_expert_product_workspace_bytes(contract_last, R, E, D0, D1)),
+                  B200MOE_ERR_WORKSPACE, "expert_product: workspace too small or not 16-byte aligned");
   B200MOE_REQUIRE(most_tiles < (int64_t{1} << 30), B200MOE_ERR_INVALID, "expert_product: too many output tiles");
   CUtensorMap cols;
   RowMaps rows;
@@ -649,12 +765,16 @@ extern "C" int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch,
     p.queue = k >= 1024 ? 2 : kQueue;
     B200MOE_CUDA_OK(cudaMemsetAsync(p.taken, 0, sizeof(int32_t), st));
   }
-  return contract_last ? launch<false, false>(cols, rows, p, most_tiles, st) : launch<false, true>(cols, rows, p, most_tiles, st);
+  const auto go = [&](auto brief) {
+    constexpr bool S = decltype(brief)::value;
+    return contract_last ? launch<false, false, S>(cols, rows, p, most_tiles, st) : launch<false, true, S>(cols, rows, p, most_tiles, st);
+  };
+  return k <= 384 ? go(std::true_type{}) : go(std::false_type{});
 }
 
 extern "C" int b200moe_expert_weight_grad(const void* a_bf16, int64_t a_pitch, const void* b_bf16, int64_t b_pitch,
                                           const int32_t* expert_offsets, int R, int E, int M, int N, void* out_bf16,
-                                          int32_t* status, b200moe_stream_t stream) {
+                                          void* workspace, size_t workspace_bytes, int32_t* status, b200moe_stream_t stream) {
   B200MOE_REQUIRE(a_bf16 && b_bf16 && expert_offsets && out_bf16 && status, B200MOE_ERR_INVALID,
                   "expert_weight_grad: null pointer argument");
   B200MOE_REQUIRE(R > 0 && E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID,
@@ -675,7 +795,13 @@ extern "C" int b200moe_expert_weight_grad(const void* a_bf16, int64_t a_pitch, c
   p.col_tiles = (N + 255) / 256;
   p.out = static_cast<__nv_bfloat16*>(out_bf16);
   p.status = status;
-  const int64_t tiles = static_cast<int64_t>(E) * p.row_tiles * p.col_tiles;
+  const int64_t tiles = weight_grad_tiles(E, M, N);
+  p.parts = split_parts(tiles, R / (static_cast<int64_t>(E) * 64));
+  p.partial = static_cast<float*>(workspace);
+  p.out_rows = static_cast<int64_t>(E) * M;
+  B200MOE_REQUIRE(p.parts == 1 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
+                                   workspace_bytes >= b200moe_expert_weight_grad_workspace_bytes(R, E, M, N)),
+                  B200MOE_ERR_WORKSPACE, "expert_weight_grad: workspace too small or not 16-byte aligned");
   B200MOE_REQUIRE(p.col_tiles < (1 << 20), B200MOE_ERR_INVALID, "expert_weight_grad: too many output columns");
   B200MOE_REQUIRE(tiles < (int64_t{1} << 30), B200MOE_ERR_INVALID, "expert_weight_grad: too many output tiles");
   p.per_matrix = make_divisor(static_cast<uint32_t>(p.row_tiles * p.col_tiles));
@@ -688,5 +814,5 @@ extern "C" int b200moe_expert_weight_grad(const void* a_bf16, int64_t a_pitch, c
   if (rc == B200MOE_OK) rc = make_map(&rows.size[3], b_bf16, N, R, b_pitch, 0, 0, 16);
   if (rc != B200MOE_OK) return rc;
   rows.size[1] = rows.size[0];  // never used
-  return launch<true, true>(cols, rows, p, tiles, static_cast<cudaStream_t>(stream));
+  return launch<true, true, false>(cols, rows, p, tiles, static_cast<cudaStream_t>(stream));
 }

@@ -228,6 +228,14 @@ def test_products_whose_tiles_are_handed_out(K, N):
     _check_product([3000, 0, 700, 1, 1299], N, K, 0, N, True)
 
 
+@pytest.mark.parametrize("counts,K,N,behind", [([5, 0, 9], 4096, 72, 3), ([300], 8200, 520, 0), ([1], 2048, 8, 0), ([40, 700, 3], 64, 12000, 5),
+                                              ([9000, 70, 0, 5003], 64, 72, 2), ([40001], 136, 8, 0)])
+def test_long_contractions_of_few_tiles(counts, K, N, behind):
+    """Contractions that are cut into parts and joined: along a weight's columns, its rows, and an expert's rows."""
+    _check_product(counts, K, N, behind, K + N, False)
+    _check_product(counts, K, N, behind, K + N, True)
+
+
 @pytest.mark.parametrize("rest", range(0, 64, 3))
 def test_weight_gradient_ends_anywhere_in_a_slab(rest):
     """The next expert's rows are inf: none of them may reach this expert's sums."""

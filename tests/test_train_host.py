@@ -29,18 +29,20 @@ def _refused(name, *args):
     ("b200moe_unsort_rows", (P, 1, 64, 4, 2, 64, P, P, 2, P, None), -1, "affinities"),
     ("b200moe_unsort_rows_backward", (P, 64, P, 64, 1, 4, 2, 64, 8, P, P, P, 0, None, None, None), -1, "null pointer"),
     ("b200moe_unsort_rows_backward", (P, 64, None, 64, 1, 4, 2, 64, 8, P, P, P, 0, None, P, None), -1, "needs rows"),
-    ("b200moe_expert_product", (P, 64, P, 64, 4096, 0, P, 8, 2, 64, 64, P, None, None), -1, "null pointer"),
-    ("b200moe_expert_product", (P, 64, P, 64, 4096, 0, P, 0, 2, 64, 64, P, P, None), -1, "one row"),
-    ("b200moe_expert_product", (P, 64, P, 64, 4096, 0, P, 8, 1025, 64, 64, P, P, None), -1, "experts"),
-    ("b200moe_expert_product", (P, 64, P, 68, 4096, 0, P, 8, 2, 64, 68, P, P, None), -1, "multiples of 8"),
-    ("b200moe_expert_product", (P, 56, P, 64, 4096, 0, P, 8, 2, 64, 64, P, P, None), -1, "16-byte boundaries"),
-    ("b200moe_expert_product", (P, 64, P + 8, 64, 4096, 0, P, 8, 2, 64, 64, P, P, None), -1, "16-byte boundaries"),
-    ("b200moe_expert_product", (P, 64, P, 64, 4100, 0, P, 8, 2, 64, 64, P, P, None), -1, "16-byte boundaries"),
-    ("b200moe_expert_product", (P, 64, P, 64, 4096, 0, P, 8, 2, 64, 64, P + 2, P, None), -1, "16-byte aligned"),
-    ("b200moe_expert_weight_grad", (P, 64, None, 64, P, 8, 2, 64, 64, P, P, None), -1, "null pointer"),
-    ("b200moe_expert_weight_grad", (P, 64, P, 64, P, 8, 2, 64, 60, P, P, None), -1, "multiples of 8"),
-    ("b200moe_expert_weight_grad", (P, 64, P, 60, P, 8, 2, 64, 64, P, P, None), -1, "16-byte boundaries"),
-    ("b200moe_expert_weight_grad", (P, 64, P, 64, P, 8, 2, 64, 64, P + 8, P, None), -1, "16-byte aligned"),
+    ("b200moe_expert_product", (P, 64, P, 64, 4096, 0, P, 8, 2, 64, 64, P, None, 0, None, None), -1, "null pointer"),
+    ("b200moe_expert_product", (P, 64, P, 64, 4096, 0, P, 0, 2, 64, 64, P, None, 0, P, None), -1, "one row"),
+    ("b200moe_expert_product", (P, 64, P, 64, 4096, 0, P, 8, 1025, 64, 64, P, None, 0, P, None), -1, "experts"),
+    ("b200moe_expert_product", (P, 64, P, 68, 4096, 0, P, 8, 2, 64, 68, P, None, 0, P, None), -1, "multiples of 8"),
+    ("b200moe_expert_product", (P, 56, P, 64, 4096, 0, P, 8, 2, 64, 64, P, None, 0, P, None), -1, "16-byte boundaries"),
+    ("b200moe_expert_product", (P, 64, P + 8, 64, 4096, 0, P, 8, 2, 64, 64, P, None, 0, P, None), -1, "16-byte boundaries"),
+    ("b200moe_expert_product", (P, 64, P, 64, 4100, 0, P, 8, 2, 64, 64, P, None, 0, P, None), -1, "16-byte boundaries"),
+    ("b200moe_expert_product", (P, 64, P, 64, 4096, 0, P, 8, 2, 64, 64, P + 2, None, 0, P, None), -1, "16-byte aligned"),
+    ("b200moe_expert_product", (P, 8192, P, 64, 1 << 19, 0, P, 8, 2, 8192, 64, P, None, 0, P, None), -3, "workspace"),
+    ("b200moe_expert_weight_grad", (P, 64, P, 64, P, 1 << 16, 2, 64, 64, P, None, 0, P, None), -3, "workspace"),
+    ("b200moe_expert_weight_grad", (P, 64, None, 64, P, 8, 2, 64, 64, P, None, 0, P, None), -1, "null pointer"),
+    ("b200moe_expert_weight_grad", (P, 64, P, 64, P, 8, 2, 64, 60, P, None, 0, P, None), -1, "multiples of 8"),
+    ("b200moe_expert_weight_grad", (P, 64, P, 60, P, 8, 2, 64, 64, P, None, 0, P, None), -1, "16-byte boundaries"),
+    ("b200moe_expert_weight_grad", (P, 64, P, 64, P, 8, 2, 64, 64, P + 8, None, 0, P, None), -1, "16-byte aligned"),
     ("b200moe_glu", (P, 64, 4, 32, 0, None, None, None, None), -1, "null pointer"),
     ("b200moe_glu", (P, 64, 4, 32, 0, P, P, None, None), -1, "null pointer"),
     ("b200moe_glu", (P, 64, 4, 28, 0, P, None, None, None), -1, "multiple of 8"),
@@ -70,9 +72,18 @@ def test_cpu_tensors_are_refused():
             call()
 
 
-def test_workspace_of_the_sort():
+def test_workspaces():
     from nki_library_b200 import _lib
     lib = _lib.load_library()
+    # few tiles of a long contraction are cut into parts, many or short ones are not
+    assert lib.b200moe_expert_product_workspace_bytes(0, 8, 2, 8192, 64) % (8 * 64 * 4) == 0
+    assert lib.b200moe_expert_product_workspace_bytes(0, 8, 2, 8192, 64) >= 2 * 8 * 64 * 4
+    assert lib.b200moe_expert_product_workspace_bytes(1, 8, 2, 64, 8192) >= 2 * 8 * 64 * 4
+    assert lib.b200moe_expert_product_workspace_bytes(0, 8, 2, 49 * 64 - 64, 64) == 0
+    assert lib.b200moe_expert_product_workspace_bytes(0, 64, 1, 4096, 4096) == 0
+    assert lib.b200moe_expert_product_workspace_bytes(0, 8192, 8, 4096, 28672) == 0
+    assert lib.b200moe_expert_weight_grad_workspace_bytes(1 << 16, 2, 64, 64) >= 2 * 2 * 64 * 64 * 4
+    assert lib.b200moe_expert_weight_grad_workspace_bytes(49 * 128 - 128, 2, 64, 64) == 0
     assert lib.b200moe_sort_workspace_bytes(1, 256) == 0
     assert lib.b200moe_sort_workspace_bytes(32768 * 8, 128) >= 128 * 4
 
