@@ -26,8 +26,8 @@ class _ExpertMLP(torch.autograd.Function):
         rows, gate_up_weight, down_weight, offsets, kept = ctx.saved_tensors
         want_rows, want_gate_up, want_down = ctx.needs_input_grad[:3]
         d_out = tile_rows(d_out)
-        d_m = product(d_out, down_weight, offsets, transpose=True)
-        d_gate_up, m = glu_backward(d_m, kept, ctx.act, want_m=want_down)
+        d_m = product(d_out, down_weight, offsets, transpose=True) if want_rows or want_gate_up else None
+        d_gate_up, m = glu_backward(d_m, kept, d_out.shape[0], down_weight.shape[1], ctx.act, want_m=want_down)
         d_down = weight_grad(m, d_out, down_weight, offsets) if want_down else None
         d_rows = product(d_gate_up, gate_up_weight, offsets, transpose=True) if want_rows else None
         d_gate_up_weight = weight_grad(rows, d_gate_up, gate_up_weight, offsets) if want_gate_up else None

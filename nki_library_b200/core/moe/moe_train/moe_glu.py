@@ -31,17 +31,20 @@ def kept_parts(kept: torch.Tensor, R: int, I: int) -> Tuple[torch.Tensor, torch.
     return kept[:R * 2 * I].view(R, 2 * I), kept[R * 2 * I:].view(R, 2, (I + 31) // 32)
 
 
-def glu_backward(d_m: torch.Tensor, kept: torch.Tensor, act: int,
-                 want_m: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """``(d_gate_up, m)`` at the kept gate and up; ``m`` None unless wanted."""
-    R, I = d_m.shape
-    d_gate_up = torch.empty((R, 2 * I), dtype=torch.bfloat16, device=d_m.device)
-    m = torch.empty((R, I), dtype=torch.bfloat16, device=d_m.device) if want_m else None
+def glu_backward(d_m: Optional[torch.Tensor], kept: torch.Tensor, R: int, I: int, act: int,
+                 want_m: bool = False) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """``(d_gate_up, m)`` at the kept gate and up; the first None without ``d_m [R, I]``, the second unless wanted."""
+    device = kept.device
+    d_gate_up = None if d_m is None else torch.empty((R, 2 * I), dtype=torch.bfloat16, device=device)
+    m = torch.empty((R, I), dtype=torch.bfloat16, device=device) if want_m else None
     if R:
-        d_m = tile_rows(d_m)
+        pitch = I
+        if d_m is not None:
+            d_m = tile_rows(d_m)
+            pitch = pitch_of(d_m)
         codes = kept.data_ptr()
-        launch(d_m.device, "b200moe_glu_backward", d_m.data_ptr(), pitch_of(d_m), codes, codes + R * 2 * I, R, I, act,
-               d_gate_up.data_ptr(), _lib.ptr(m))
+        launch(device, "b200moe_glu_backward", _lib.ptr(d_m), pitch, codes, codes + R * 2 * I, R, I, act, _lib.ptr(d_gate_up),
+               _lib.ptr(m))
     return d_gate_up, m
 
 
@@ -57,7 +60,7 @@ class _Glu(torch.autograd.Function):
     @once
     def backward(ctx, d_m):
         kept, = ctx.saved_tensors
-        return glu_backward(d_m, kept, ctx.act)[0], None
+        return glu_backward(d_m, kept, *d_m.shape, ctx.act)[0], None
 
 
 def moe_glu(gate_up: torch.Tensor, activation_function: ActFnType = ActFnType.SiLU) -> torch.Tensor:

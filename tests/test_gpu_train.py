@@ -395,7 +395,7 @@ def test_checkpoint_is_exact(I):
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
     # and what the backward pass makes of it: m from the kept values
     with torch.no_grad():
-        _, again = glu_backward(torch.ones((R, I), device="cuda").bfloat16(), checkpoint, 0, want_m=True)
+        _, again = glu_backward(None, checkpoint, R, I, 0, want_m=True)
     a, _ = ref.act_and_slope(g, "SiLU")
     want = a * u
     rows = want.abs().amax(1) < 1e30  # also drops rows with NaN
@@ -474,7 +474,7 @@ def test_layer_is_its_operators(T, K, E, H, I, dropped):
         assert torch.equal(g, w)
     with torch.no_grad():
         _, checkpoint = glu_forward(gate_up, 0, True)
-        _, m_kept = glu_backward(act, checkpoint, 0, want_m=True)
+        _, m_kept = glu_backward(None, checkpoint, *act.shape, 0, want_m=True)
         assert torch.equal(grads[3], weight_grad(m_kept, d_y, w2, plan.expert_offsets))
         assert torch.equal(m.moe_experts_train(*(t.detach() if t.is_floating_point() else t for t in (hidden, aff)), idx,
                                                w1.detach(), w2.detach()), out)
@@ -537,6 +537,44 @@ def test_runs_repeat_bit_for_bit_and_on_other_streams():
     torch.cuda.synchronize()
     for got in results:
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# handed-out tiles, parts that are joined, and the fixed walk: counts, K, N
+FORMS = [([3000, 700, 1296], 128, 7680), ([40, 24], 4096, 64), ([9000, 70, 5003], 64, 72), ([100, 28], 256, 520)]
+
+
+@pytest.mark.parametrize("counts,K,N", FORMS)
+def test_every_form_of_the_products_is_captured_and_runs_beside_another(counts, K, N):
+    """Two graphs of the same product and gradients, replayed in turn and on two streams at once, between eager calls."""
+    import nki_library_b200 as m
+    offsets, x, w, dy = _product_case(counts, K, N, 2, K)
+    x[sum(counts):], dy[sum(counts):] = 0, 0
+    x.requires_grad_(), w.requires_grad_()
+
+    def step():
+        y = m.expert_linear(x, w, offsets)
+        return (y.detach(), *torch.autograd.grad(y, (x, w), dy))
+
+    want = step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results = step()
+        graphs.append((graph, results))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for (graph, results), stream in zip(graphs, streams):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                for r in results:
+                    r.fill_(7)
+                graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        for got in (eager, *(r for _, r in graphs)):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_first_call_of_a_thread():
