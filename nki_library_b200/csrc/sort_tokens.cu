@@ -7,6 +7,7 @@
 #include "common.cuh"
 #include "quantize_row.cuh"
 
+#include <initializer_list>
 #include <type_traits>
 
 namespace b200moe {
@@ -156,46 +157,57 @@ __global__ void __launch_bounds__(kSortThreads) place_pairs_kernel(SortArgs a, c
 }
 
 // ------------------------------------------------------------------ rows
-// The elements of a row that a thread holds at once, `chunk` by `chunk` of the CTA's: 16 consecutive bytes, or, where rows are
-// not made of whole aligned 16 bytes, eight elements a CTA's width apart.
-template <typename T, bool WIDE>
+// The elements of a row that a thread holds at once, `chunk` by `chunk` of the CTA's: one unit of 16 bytes, or, where rows are
+// not made of whole aligned 16 bytes, a few units of 4 or 2 bytes a CTA's width apart.
+template <typename T, int UNIT>
 struct Piece {
-  static constexpr int kCount = WIDE ? 16 / static_cast<int>(sizeof(T)) : 8;
-  uint32_t raw[WIDE ? 4 : 8];
+  static constexpr int kUnits = UNIT == 16 ? 1 : 4;  // eight: 252 us for that sum, 804 instead of 317 for its gradients
+  static constexpr int kPer = UNIT / static_cast<int>(sizeof(T));  // elements of a unit
+  static constexpr int kCount = kUnits * kPer;
+  uint32_t raw[UNIT == 16 ? 4 : kUnits];
 
   __device__ __forceinline__ static int chunk() { return static_cast<int>(blockDim.x) * kCount; }
-  // Index of element i of the chunk that starts at h; those at H and behind do not exist.
-  __device__ __forceinline__ static int index(int h, int i) {
-    return WIDE ? h + static_cast<int>(threadIdx.x) * kCount + i : h + i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x);
+  // Index of the first element of unit u of the chunk that starts at h; units at H and behind do not exist.
+  __device__ __forceinline__ static int index(int h, int u) {
+    return h + (u * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * kPer;
   }
+  // Only loads, so that a caller's next row is asked for before this one is there (shifting 2-byte units on the spot took 387 us
+  // instead of 187 for the sum of 48000 rows of 5003).
   __device__ __forceinline__ void fetch(const T* row, int h, int H) {
-    if constexpr (WIDE) {
-      if (index(h, 0) < H) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + index(h, 0)));
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      if (index(h, u) >= H) {
+        raw[u] = 0;
+        if constexpr (UNIT == 16) raw[1] = raw[2] = raw[3] = 0;
+        continue;
+      }
+      const T* p = row + index(h, u);
+      if constexpr (UNIT == 16) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
         raw[0] = v.x; raw[1] = v.y; raw[2] = v.z; raw[3] = v.w;
+      } else if constexpr (UNIT == 4) raw[u] = __ldg(reinterpret_cast<const uint32_t*>(p));
+      else raw[u] = __ldg(reinterpret_cast<const uint16_t*>(p));
+    }
+  }
+  // Zero in units that do not exist.
+  __device__ __forceinline__ void values(float (&v)[kCount]) const {
+    if constexpr (sizeof(T) == 2 && UNIT > 2) {
+#pragma unroll
+      for (int i = 0; i < kCount / 2; ++i) {
+        v[2 * i] = __uint_as_float(raw[i] << 16);
+        v[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < kCount; ++i) {
-        if (index(h, i) >= H) continue;
-        if constexpr (sizeof(T) == 2) raw[i] = static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(row) + index(h, i))) << 16;
-        else raw[i] = __ldg(reinterpret_cast<const uint32_t*>(row) + index(h, i));
-      }
-    }
-  }
-  __device__ __forceinline__ void values(float (&v)[kCount]) const {
-    if constexpr (WIDE && sizeof(T) == 2) unpack8_bf16(make_uint4(raw[0], raw[1], raw[2], raw[3]), v);
-    else {
-#pragma unroll
-      for (int i = 0; i < kCount; ++i) v[i] = __uint_as_float(raw[i]);
+      for (int i = 0; i < kCount; ++i) v[i] = __uint_as_float(sizeof(T) == 2 ? raw[i] << 16 : raw[i]);
     }
   }
   __device__ __forceinline__ static void store(T* row, int h, int H, const float (&v)[kCount]) {
-    if constexpr (WIDE) {
-      if (index(h, 0) >= H) return;
-      uint32_t w[4];
+    constexpr int kWords = kCount * static_cast<int>(sizeof(T)) / 4;
+    uint32_t w[kWords > 0 ? kWords : 1];
+    if constexpr (UNIT > 2) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kWords; ++i) {
         if constexpr (sizeof(T) == 2) {
           const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
           w[i] = *reinterpret_cast<const uint32_t*>(&b);
@@ -203,11 +215,14 @@ struct Piece {
           w[i] = __float_as_uint(v[i]);
         }
       }
-      *reinterpret_cast<uint4*>(row + index(h, 0)) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
+    }
 #pragma unroll
-      for (int i = 0; i < kCount; ++i)
-        if (index(h, i) < H) row[index(h, i)] = static_cast<T>(v[i]);
+    for (int u = 0; u < kUnits; ++u) {
+      if (index(h, u) >= H) continue;
+      T* p = row + index(h, u);
+      if constexpr (UNIT == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+      else if constexpr (UNIT == 4) *reinterpret_cast<uint32_t*>(p) = w[u];
+      else *p = static_cast<T>(v[u]);
     }
   }
 };
@@ -231,9 +246,9 @@ __device__ __forceinline__ int64_t own_token() {
 }
 
 // The K rows that a token's threads clear if they lie behind the last expert's: rows t * K to t * K + K - 1.
-template <typename T, bool WIDE>
+template <typename T, int UNIT>
 __device__ __forceinline__ void clear_rows_behind(const RowArgs& a, int64_t t, T* rows) {
-  using P = Piece<T, WIDE>;
+  using P = Piece<T, UNIT>;
   const int64_t r0 = t * a.K;
   const float zero[P::kCount] = {};
   for (int64_t r = max(r0, static_cast<int64_t>(a.offsets[a.E])); r < r0 + a.K; ++r)
@@ -241,9 +256,9 @@ __device__ __forceinline__ void clear_rows_behind(const RowArgs& a, int64_t t, T
 }
 
 // rows[row_of_pair[t, k]] = hidden[t].  32768 tokens x 4096 bf16, top-8: 2.4 GB in 396 us, the copy rate.
-template <typename T, bool WIDE, bool SHORT>
+template <typename T, int UNIT, bool SHORT>
 __global__ void __launch_bounds__(128) sort_rows_kernel(RowArgs a, const T* hidden, int64_t pitch, T* rows) {
-  using P = Piece<T, WIDE>;
+  using P = Piece<T, UNIT>;
   grid_enter(a.row_of_pair, a.offsets, hidden);
   const int64_t t = own_token<SHORT>();
   if (SHORT && t >= a.T) return;
@@ -257,15 +272,15 @@ __global__ void __launch_bounds__(128) sort_rows_kernel(RowArgs a, const T* hidd
       if (r >= 0) P::store(rows + r * a.H, h, a.H, v);
     }
   }
-  clear_rows_behind<T, WIDE>(a, t, rows);
+  clear_rows_behind<T, UNIT>(a, t, rows);
 }
 
 // out[t] = sum over k of (affinities[t, k]) rows[row_of_pair[t, k]], in fp32, k ascending, rounded once.  The same 2.4 GB in
 // 356 us (343 without weights); one row at a time, 400 (386).
-template <typename T, bool WIDE, bool SHORT, int ROWS>
+template <typename T, int UNIT, bool SHORT, int ROWS>
 __global__ void __launch_bounds__(128) unsort_rows_kernel(RowArgs a, const T* rows, int64_t pitch, const void* affinities,
                                                           int aff_dtype, T* out) {
-  using P = Piece<T, WIDE>;
+  using P = Piece<T, UNIT>;
   grid_enter(a.row_of_pair, rows, affinities);
   const int64_t t = own_token<SHORT>();
   if (SHORT && t >= a.T) return;
@@ -298,11 +313,11 @@ __global__ void __launch_bounds__(128) unsort_rows_kernel(RowArgs a, const T* ro
 
 // d rows[r] = a[t, k] d out[t]; d a[t, k] = <d out[t], rows[r]>: one pass over a token's rows for both.  32768 tokens x 4096
 // bf16, top-8: 4.6 GB in 695 us; with a row's load, product and store one after the other 1121.
-template <typename T, bool WIDE, bool SHORT, int ROWS>
+template <typename T, int UNIT, bool SHORT, int ROWS>
 __global__ void __launch_bounds__(256) unsort_backward_kernel(RowArgs a, const T* d_out, int64_t d_pitch, const T* rows,
                                                               int64_t pitch, const void* affinities, int aff_dtype,
                                                               T* d_rows, void* d_affinities) {
-  using P = Piece<T, WIDE>;
+  using P = Piece<T, UNIT>;
   __shared__ float s_dot[8][ROWS];
   grid_enter(a.row_of_pair, a.offsets, d_out, rows, affinities);
   const int64_t t = own_token<SHORT>();
@@ -335,8 +350,7 @@ __global__ void __launch_bounds__(256) unsort_backward_kernel(RowArgs a, const T
         if (d_affinities != nullptr) {
           piece[j].values(v);
 #pragma unroll
-          for (int i = 0; i < P::kCount; ++i)
-            if (P::index(h, i) < a.H) dot[j] = fmaf(d[i], v[i], dot[j]);
+          for (int i = 0; i < P::kCount; ++i) dot[j] = fmaf(d[i], v[i], dot[j]);
         }
         if (d_rows != nullptr) {
 #pragma unroll
@@ -362,11 +376,20 @@ __global__ void __launch_bounds__(256) unsort_backward_kernel(RowArgs a, const T
       __syncthreads();
     }
   }
-  if (d_rows != nullptr && (!SHORT || t < a.T)) clear_rows_behind<T, WIDE>(a, t, d_rows);
+  if (d_rows != nullptr && (!SHORT || t < a.T)) clear_rows_behind<T, UNIT>(a, t, d_rows);
 }
 
-bool whole_vectors(const void* p, int64_t pitch_bytes) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && pitch_bytes % 16 == 0;
+// Bytes that the rows of all given matrices can be moved by: 16, 4, or an element's.
+struct Rows {
+  const void* p;
+  int64_t pitch;
+};
+int common_unit(int dtype, int H, std::initializer_list<Rows> matrices) {
+  const int size = dtype == B200MOE_F32 ? 4 : 2;
+  uint64_t bits = static_cast<uint64_t>(H) * size;
+  for (const Rows& m : matrices)
+    if (m.p != nullptr) bits |= reinterpret_cast<uintptr_t>(m.p) | static_cast<uint64_t>(m.pitch * size);
+  return bits % 16 == 0 ? 16 : (bits % 4 == 0 ? 4 : size);
 }
 
 // With enough tokens to give every SM several CTAs, a CTA of `threads` has as many tokens as their rows leave room for (30000
@@ -393,11 +416,14 @@ int check_rows(const char* name, int dtype, int T, int K, int H, int64_t pitch) 
   return B200MOE_OK;
 }
 
-// Calls fn with a value of the element type and whether its rows move 16 bytes at a time, both known to the compiler.
+// Calls fn with a value of the element type and the unit its rows move by, both known to the compiler.
 template <typename F>
-int with_rows(int dtype, bool wide, const F& fn) {
-  if (dtype == B200MOE_BF16) return wide ? fn(__nv_bfloat16{}, std::true_type{}) : fn(__nv_bfloat16{}, std::false_type{});
-  return wide ? fn(float{}, std::true_type{}) : fn(float{}, std::false_type{});
+int with_rows(int dtype, int unit, const F& fn) {
+  using std::integral_constant;
+  if (dtype == B200MOE_F32)
+    return unit == 16 ? fn(float{}, integral_constant<int, 16>{}) : fn(float{}, integral_constant<int, 4>{});
+  if (unit == 16) return fn(__nv_bfloat16{}, integral_constant<int, 16>{});
+  return unit == 4 ? fn(__nv_bfloat16{}, integral_constant<int, 4>{}) : fn(__nv_bfloat16{}, integral_constant<int, 2>{});
 }
 
 }  // namespace
@@ -444,13 +470,11 @@ extern "C" int b200moe_sort_rows(const void* hidden, int dtype, int64_t pitch, i
   if (rc != B200MOE_OK) return rc;
   B200MOE_REQUIRE(E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID, "sort_rows: between 1 and %d experts, got %d", kMaxExperts, E);
   const RowArgs a{T, K, H, E, row_of_pair, expert_offsets};
-  const int size = dtype == B200MOE_F32 ? 4 : 2;
-  const bool wide = whole_vectors(hidden, pitch * size) && whole_vectors(rows, static_cast<int64_t>(H) * size);
-  return with_rows(dtype, wide, [&](auto element, auto width) -> int {
+  return with_rows(dtype, common_unit(dtype, H, {{hidden, pitch}, {rows, H}}), [&](auto element, auto width) -> int {
     using T_ = decltype(element);
-    constexpr bool W = decltype(width)::value;
-    const Layout l = row_layout(T, H, Piece<T_, W>::kCount, 128, true);
-    const auto kernel = l.block.y > 1 ? sort_rows_kernel<T_, W, true> : sort_rows_kernel<T_, W, false>;
+    constexpr int U = decltype(width)::value;
+    const Layout l = row_layout(T, H, Piece<T_, U>::kCount, 128, true);
+    const auto kernel = l.block.y > 1 ? sort_rows_kernel<T_, U, true> : sort_rows_kernel<T_, U, false>;
     B200MOE_CUDA_OK(launch_overlapped(kernel, l.grid, l.block, 0, static_cast<cudaStream_t>(stream), a,
                                       static_cast<const T_*>(hidden), pitch, static_cast<T_*>(rows)));
     B200MOE_LAUNCH_OK("sort_rows_kernel");
@@ -476,14 +500,12 @@ extern "C" int b200moe_unsort_rows(const void* rows, int dtype, int64_t pitch, i
   B200MOE_REQUIRE(affinities == nullptr || aff_dtype == B200MOE_F32 || aff_dtype == B200MOE_BF16, B200MOE_ERR_INVALID,
                   "unsort_rows: affinities must be fp32 or bf16");
   const RowArgs a{T, K, H, 0, row_of_pair, nullptr};
-  const int size = dtype == B200MOE_F32 ? 4 : 2;
-  const bool wide = whole_vectors(rows, pitch * size) && whole_vectors(out, static_cast<int64_t>(H) * size);
-  return with_rows(dtype, wide, [&](auto element, auto width) -> int {
+  return with_rows(dtype, common_unit(dtype, H, {{rows, pitch}, {out, H}}), [&](auto element, auto width) -> int {
     using T_ = decltype(element);
-    constexpr bool W = decltype(width)::value;
-    const Layout l = row_layout(T, H, Piece<T_, W>::kCount, 128, true);
-    const auto kernel = l.block.y > 1 ? (K > 4 ? unsort_rows_kernel<T_, W, true, 8> : unsort_rows_kernel<T_, W, true, 4>)
-                                      : (K > 4 ? unsort_rows_kernel<T_, W, false, 8> : unsort_rows_kernel<T_, W, false, 4>);
+    constexpr int U = decltype(width)::value;
+    const Layout l = row_layout(T, H, Piece<T_, U>::kCount, 128, true);
+    const auto kernel = l.block.y > 1 ? (K > 4 ? unsort_rows_kernel<T_, U, true, 8> : unsort_rows_kernel<T_, U, true, 4>)
+                                      : (K > 4 ? unsort_rows_kernel<T_, U, false, 8> : unsort_rows_kernel<T_, U, false, 4>);
     B200MOE_CUDA_OK(launch_overlapped(kernel, l.grid, l.block, 0, static_cast<cudaStream_t>(stream), a,
                                       static_cast<const T_*>(rows), pitch, affinities, aff_dtype, static_cast<T_*>(out)));
     B200MOE_LAUNCH_OK("unsort_rows_kernel");
@@ -507,19 +529,15 @@ extern "C" int b200moe_unsort_rows_backward(const void* d_out, int64_t d_pitch, 
   B200MOE_REQUIRE(E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID, "unsort_rows_backward: between 1 and %d experts, got %d",
                   kMaxExperts, E);
   const RowArgs a{T, K, H, E, row_of_pair, expert_offsets};
-  const int size = dtype == B200MOE_F32 ? 4 : 2;
-  const bool wide = whole_vectors(d_out, d_pitch * size) && (rows == nullptr || whole_vectors(rows, pitch * size)) &&
-                    (d_rows == nullptr || whole_vectors(d_rows, static_cast<int64_t>(H) * size)) &&
-                    static_cast<int64_t>(H) * size % 16 == 0;
-  return with_rows(dtype, wide, [&](auto element, auto width) -> int {
+  return with_rows(dtype, common_unit(dtype, H, {{d_out, d_pitch}, {rows, pitch}, {d_rows, H}}), [&](auto element, auto width) -> int {
     using T_ = decltype(element);
-    constexpr bool W = decltype(width)::value;
-    const int threads = T >= 8 * sm_count() && H <= 128 * 4 * Piece<T_, W>::kCount ? 128 : 256;
-    const Layout l = row_layout(T, H, Piece<T_, W>::kCount, threads, false);
+    constexpr int U = decltype(width)::value;
+    const int threads = T >= 8 * sm_count() && H <= 128 * 4 * Piece<T_, U>::kCount ? 128 : 256;
+    const Layout l = row_layout(T, H, Piece<T_, U>::kCount, threads, false);
     const auto pick = [&](auto few) {
       constexpr bool S = decltype(few)::value;
-      return K > 4 ? unsort_backward_kernel<T_, W, S, 8>
-                   : (K > 2 ? unsort_backward_kernel<T_, W, S, 4> : unsort_backward_kernel<T_, W, S, 2>);
+      return K > 4 ? unsort_backward_kernel<T_, U, S, 8>
+                   : (K > 2 ? unsort_backward_kernel<T_, U, S, 4> : unsort_backward_kernel<T_, U, S, 2>);
     };
     const auto kernel = l.block.y > 1 ? pick(std::true_type{}) : pick(std::false_type{});
     B200MOE_CUDA_OK(launch_overlapped(kernel, l.grid, l.block, 0, static_cast<cudaStream_t>(stream), a,
