@@ -83,8 +83,8 @@ struct Sched {
 };
 
 // Epilogue groups of four warps: one for a product, whose stores pass while the next tile's contraction runs, two where that is
-// as short as the stores (SHORT; 9216 rows on 6 experts of K x 13376, one group / two: K 64 87 / 73 us, 256 92 / 81; of 512 x 8192
-// 69 / 70, 4096 x 4096 212 / 214) and for the weight grad.
+// as short as the stores (SHORT; 9216 rows on 6 experts of K x 13376, one group / two: K 64 79 / 64 us, 256 85 / 72; of 512 x 8192
+// 68 / 68) and for the weight grad.
 template <bool WGRAD, bool SHORT>
 struct Config {
   static constexpr int kGroups = WGRAD || SHORT ? 2 : 1;
@@ -757,10 +757,12 @@ extern "C" int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch,
   // Row tiles of an expert share its weight tiles in L2 as long as they run side by side.  A fixed walk drifts apart, since
   // tiles differ in width; handed out in order as pairs come free they stay together (32 experts of 7168 x 4096, 32768
   // rows, skewed: 5.6 -> 2.8 GB from DRAM, 1533 -> 1356 us; its row gradient 3.6 -> 2.4 GB, 1440 -> 1342 us).  With one row
-  // tile per expert there is nothing to share, and the counter's memset and the queue cost more than they bring (64 experts
-  // of 2048 x 2048, 125 rows each: 109 us without, 118 with); so they do for the weight gradient's short contractions (4 x 1024
+  // tile per expert there is nothing to share, and with operands that L2 holds nothing to lose, while the counter's memset and
+  // the queue cost 4 to 9 us (64 experts of 2048 x 2048, 125 rows each: 109 us without, 118 with; 9216 rows on 6 experts of
+  // 64 x 13376: 64 and 73, of 4096 x 4096 211 and 215); so they do for the weight gradient's short contractions (4 x 1024
   // rows, 4096 x 14336: 353 and 367 us).
-  if (R >= 512 * static_cast<int64_t>(E) && most_tiles >= 4 * (sm_count() / 2)) {
+  const int64_t bytes = 2 * (static_cast<int64_t>(E) * D0 * D1 + static_cast<int64_t>(R) * (static_cast<int64_t>(D0) + D1));
+  if (R >= 512 * static_cast<int64_t>(E) && bytes >= (int64_t{1} << 29) && most_tiles >= 4 * (sm_count() / 2)) {
     p.taken = status + 1;
     p.queue = k >= 1024 ? 2 : kQueue;
     B200MOE_CUDA_OK(cudaMemsetAsync(p.taken, 0, sizeof(int32_t), st));

@@ -221,11 +221,11 @@ def test_products(counts, K, N, behind, transposed):
     _check_product(COUNTS[counts], K, N, behind, K + N, transposed)
 
 
-@pytest.mark.parametrize("K,N", [(72, 7688), (1032, 7680), (64, 15000)])
+@pytest.mark.parametrize("K,N", [(72, 14008), (1032, 13000)])
 def test_products_whose_tiles_are_handed_out(K, N):
-    """Enough rows per expert and tiles for the pairs to draw their tiles from one counter."""
-    _check_product([3000, 0, 700, 1, 1299], K, N, 40, K, False)
-    _check_product([3000, 0, 700, 1, 1299], N, K, 0, N, True)
+    """Rows per expert, bytes and tiles enough for the pairs to draw their tiles from one counter."""
+    _check_product([12000, 0, 3000, 1, 5199], K, N, 40, K, False)
+    _check_product([12000, 0, 3000, 1, 5199], N, K, 0, N, True)
 
 
 @pytest.mark.parametrize("counts,K,N,behind", [([5, 0, 9], 4096, 72, 3), ([300], 8200, 520, 0), ([1], 2048, 8, 0), ([40, 700, 3], 64, 12000, 5),
@@ -540,7 +540,7 @@ def test_runs_repeat_bit_for_bit_and_on_other_streams():
 
 
 # handed-out tiles, parts that are joined, and the fixed walk: counts, K, N
-FORMS = [([3000, 700, 1296], 128, 7680), ([40, 24], 4096, 64), ([9000, 70, 5003], 64, 72), ([100, 28], 256, 520)]
+FORMS = [([12000, 5000, 3240], 128, 14000), ([40, 24], 4096, 64), ([9000, 70, 5003], 64, 72), ([100, 28], 256, 520)]
 
 
 @pytest.mark.parametrize("counts,K,N", FORMS)
