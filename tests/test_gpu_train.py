@@ -221,6 +221,10 @@ def test_products(counts, K, N, behind, transposed):
     _check_product(COUNTS[counts], K, N, behind, K + N, transposed)
 
 
+def test_products_of_the_most_experts():
+    _check_product([(5 * e) % 3 for e in range(1024)], 40, 72, 0, 3, False)
+
+
 @pytest.mark.parametrize("K,N", [(72, 14008), (1032, 13000)])
 def test_products_whose_tiles_are_handed_out(K, N):
     """Rows per expert, bytes and tiles enough for the pairs to draw their tiles from one counter."""
