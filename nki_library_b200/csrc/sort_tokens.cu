@@ -33,6 +33,7 @@ __device__ __forceinline__ int expert_of(const SortArgs& a, int64_t p) {
 }
 
 constexpr int kRounds = kSpan / 32;
+constexpr int kMostHist = (kSortWarps + 1) * kMaxExperts * static_cast<int>(sizeof(int));
 
 // How many pairs of each expert a chunk has; no order in it, so atomics on shared memory do.
 __global__ void __launch_bounds__(kSortThreads) count_pairs_kernel(SortArgs a, int* chunk_counts) {
@@ -51,16 +52,15 @@ __global__ void __launch_bounds__(kSortThreads) count_pairs_kernel(SortArgs a, i
   for (int e = threadIdx.x; e < a.E; e += kSortThreads) chunk_counts[static_cast<int64_t>(blockIdx.x) * a.E + e] = hist[e];
 }
 
-// Every CTA adds the chunks' counts up for itself: its own base per expert costs no third launch.
-__global__ void __launch_bounds__(kSortThreads) place_pairs_kernel(SortArgs a, const int* chunk_counts, int32_t* offsets,
-                                                                   int32_t* row_of_pair) {
-  extern __shared__ int hist[];  // [kSortWarps][E], then base [E]
+// Rows of one chunk's pairs, by a whole CTA; `put(pair, row)` is called once per pair, -1 for none.  Every CTA adds the chunks'
+// counts up for itself: its own base per expert costs no third launch.  Returns the number of rows; `offsets` may be NULL.
+template <typename Put>
+__device__ __forceinline__ int order_chunk(const SortArgs& a, int chunk, int chunks, const int* chunk_counts, int* hist,
+                                           int32_t* offsets, const Put& put) {
   __shared__ int s_warp[kSortWarps], s_before[kSortThreads], s_total[kSortThreads];
-  grid_enter(a.index, chunk_counts);
-  int* base = hist + kSortWarps * a.E;
-  const int64_t p0 = static_cast<int64_t>(blockIdx.x) * kChunk;
+  int* base = hist + kSortWarps * a.E;  // hist [kSortWarps][E], then base [E]
+  const int64_t p0 = static_cast<int64_t>(chunk) * kChunk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int chunks = gridDim.x;
   // a lane's pairs, its lanes of equal expert in each round, and hist[w * E + e] = pairs of expert e among warp w's
   int expert[kRounds];
   unsigned same[kRounds];
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kSortThreads) place_pairs_kernel(SortArgs a, c
 #pragma unroll 16
         for (int c = part; c < chunks; c += parts) {
           const int n = chunk_counts[static_cast<int64_t>(c) * a.E + e];
-          before += c < static_cast<int>(blockIdx.x) ? n : 0;
+          before += c < chunk ? n : 0;
           total += n;
         }
       }
@@ -126,12 +126,12 @@ __global__ void __launch_bounds__(kSortThreads) place_pairs_kernel(SortArgs a, c
       run += s_warp[w];
     }
     if (part == 0 && e < a.E) {
-      if (blockIdx.x == 0) offsets[e] = first;
+      if (offsets != nullptr) offsets[e] = first;
       base[e] = first + before;
     }
     __syncthreads();
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) offsets[a.E] = run;
+  if (offsets != nullptr && threadIdx.x == 0) offsets[a.E] = run;
   // a warp's part of an expert follows those of the warps before it
   for (int e = threadIdx.x; e < a.E; e += kSortThreads) {
     int at = base[e];
@@ -152,8 +152,17 @@ __global__ void __launch_bounds__(kSortThreads) place_pairs_kernel(SortArgs a, c
     __syncwarp();
     if (e >= 0 && lane == __ffs(same[i]) - 1) hist[warp * a.E + e] = at + __popc(same[i]);
     __syncwarp();
-    if (p < a.pairs) row_of_pair[p] = row;
+    if (p < a.pairs) put(p, row);
   }
+  return run;
+}
+
+__global__ void __launch_bounds__(kSortThreads) place_pairs_kernel(SortArgs a, const int* chunk_counts, int32_t* offsets,
+                                                                   int32_t* row_of_pair) {
+  extern __shared__ int hist[];
+  grid_enter(a.index, chunk_counts);
+  order_chunk(a, blockIdx.x, gridDim.x, chunk_counts, hist, blockIdx.x == 0 ? offsets : nullptr,
+              [&](int64_t p, int row) { row_of_pair[p] = row; });
 }
 
 // ------------------------------------------------------------------ rows
@@ -273,6 +282,36 @@ __global__ void __launch_bounds__(128) sort_rows_kernel(RowArgs a, const T* hidd
     }
   }
   clear_rows_behind<T, UNIT>(a, t, rows);
+}
+
+// Order and rows in one launch for a few tokens: every CTA works the order out for itself and moves one token's rows.
+template <typename T, int UNIT>
+__global__ void __launch_bounds__(kSortThreads) sort_few_kernel(SortArgs s, RowArgs a, const T* hidden, int64_t pitch,
+                                                                int32_t* offsets, int32_t* row_of_pair, T* rows) {
+  using P = Piece<T, UNIT>;
+  extern __shared__ int hist[];
+  __shared__ int s_row[kChunk];
+  grid_enter(s.index, hidden);
+  const bool first = blockIdx.x == 0;
+  const int64_t t = blockIdx.x;
+  P piece;  // on its way while the order is worked out
+  piece.fetch(hidden + t * pitch, 0, a.H);
+  const int used = order_chunk(s, 0, 1, nullptr, hist, first ? offsets : nullptr, [&](int64_t p, int row) {
+    s_row[p] = row;
+    if (first) row_of_pair[p] = row;
+  });
+  __syncthreads();
+  const float zero[P::kCount] = {};
+  for (int h = 0; h < a.H; h += P::chunk()) {
+    float v[P::kCount];
+    if (h > 0) piece.fetch(hidden + t * pitch, h, a.H);
+    piece.values(v);
+    for (int k = 0; k < a.K; ++k) {
+      const int r = s_row[t * a.K + k];
+      if (r >= 0) P::store(rows + static_cast<int64_t>(r) * a.H, h, a.H, v);
+      if (t * a.K + k >= used) P::store(rows + (t * a.K + k) * a.H, h, a.H, zero);  // this row lies behind the last expert's
+    }
+  }
 }
 
 // out[t] = sum over k of (affinities[t, k]) rows[row_of_pair[t, k]], in fp32, k ascending, rounded once.  The same 2.4 GB in
@@ -416,6 +455,16 @@ int check_rows(const char* name, int dtype, int T, int K, int H, int64_t pitch) 
   return B200MOE_OK;
 }
 
+int check_sort(const void* expert_index, int index_bytes, int T, int K, int E, const int32_t* expert_offsets,
+               const int32_t* row_of_pair) {
+  B200MOE_REQUIRE(expert_index && expert_offsets && row_of_pair, B200MOE_ERR_INVALID, "sort_pairs: null pointer argument");
+  B200MOE_REQUIRE(index_bytes == 4 || index_bytes == 8, B200MOE_ERR_INVALID, "sort_pairs: ids must have 4 or 8 bytes");
+  B200MOE_REQUIRE(T > 0 && K > 0 && static_cast<int64_t>(T) * K <= INT32_MAX, B200MOE_ERR_INVALID,
+                  "sort_pairs: need T, K > 0 and at most 2^31 - 1 pairs");
+  B200MOE_REQUIRE(E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID, "sort_pairs: between 1 and %d experts, got %d", kMaxExperts, E);
+  return B200MOE_OK;
+}
+
 // Calls fn with a value of the element type and the unit its rows move by, both known to the compiler.
 template <typename F>
 int with_rows(int dtype, int unit, const F& fn) {
@@ -438,11 +487,8 @@ extern "C" size_t b200moe_sort_workspace_bytes(int64_t pairs, int E) {
 
 extern "C" int b200moe_sort_pairs(const void* expert_index, int index_bytes, int T, int K, int E, int32_t* expert_offsets,
                                   int32_t* row_of_pair, void* workspace, size_t workspace_bytes, b200moe_stream_t stream) {
-  B200MOE_REQUIRE(expert_index && expert_offsets && row_of_pair, B200MOE_ERR_INVALID, "sort_pairs: null pointer argument");
-  B200MOE_REQUIRE(index_bytes == 4 || index_bytes == 8, B200MOE_ERR_INVALID, "sort_pairs: ids must have 4 or 8 bytes");
-  B200MOE_REQUIRE(T > 0 && K > 0 && static_cast<int64_t>(T) * K <= INT32_MAX, B200MOE_ERR_INVALID,
-                  "sort_pairs: need T, K > 0 and at most 2^31 - 1 pairs");
-  B200MOE_REQUIRE(E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID, "sort_pairs: between 1 and %d experts, got %d", kMaxExperts, E);
+  const int rc = check_sort(expert_index, index_bytes, T, K, E, expert_offsets, row_of_pair);
+  if (rc != B200MOE_OK) return rc;
   const SortArgs a{expert_index, index_bytes == 8, static_cast<int64_t>(T) * K, E};
   const int64_t chunks = ceil_div64(a.pairs, kChunk);
   B200MOE_REQUIRE(chunks == 1 || (workspace != nullptr && workspace_bytes >= b200moe_sort_workspace_bytes(a.pairs, E)),
@@ -454,8 +500,7 @@ extern "C" int b200moe_sort_pairs(const void* expert_index, int index_bytes, int
     B200MOE_CUDA_OK(launch_overlapped(count_pairs_kernel, grid, kSortThreads, E * sizeof(int), st, a, static_cast<int*>(workspace)));
     B200MOE_LAUNCH_OK("count_pairs_kernel");
   }
-  B200MOE_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(place_pairs_kernel),
-                                      (kSortWarps + 1) * kMaxExperts * static_cast<int>(sizeof(int))));
+  B200MOE_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(place_pairs_kernel), kMostHist));
   B200MOE_CUDA_OK(launch_overlapped(place_pairs_kernel, grid, kSortThreads, hist, st, a,
                                     static_cast<const int*>(workspace), expert_offsets, row_of_pair));
   B200MOE_LAUNCH_OK("place_pairs_kernel");
@@ -487,7 +532,26 @@ extern "C" int b200moe_sort_tokens(const void* hidden, int dtype, int64_t pitch,
                                    void* workspace, size_t workspace_bytes, b200moe_stream_t stream) {
   B200MOE_REQUIRE(hidden && rows, B200MOE_ERR_INVALID, "sort_tokens: null pointer argument");
   int rc = check_rows("sort_tokens", dtype, T, K, H, pitch);
-  if (rc == B200MOE_OK) rc = b200moe_sort_pairs(expert_index, index_bytes, T, K, E, expert_offsets, row_of_pair, workspace, workspace_bytes, stream);
+  if (rc != B200MOE_OK) return rc;
+  rc = check_sort(expert_index, index_bytes, T, K, E, expert_offsets, row_of_pair);
+  if (rc != B200MOE_OK) return rc;
+  // One launch instead of two where a CTA per token does not repeat the order too often (16 tokens of 4096, 128 experts, top-8: 7.0 us
+  // instead of 4.8 + 3.8, and 16.6 instead of 19.3 of host time)
+  if (static_cast<int64_t>(T) * K <= kChunk && T <= 128) {
+    const SortArgs s{expert_index, index_bytes == 8, static_cast<int64_t>(T) * K, E};
+    const RowArgs a{T, K, H, E, nullptr, nullptr};
+    return with_rows(dtype, common_unit(dtype, H, {{hidden, pitch}, {rows, H}}), [&](auto element, auto width) -> int {
+      using T_ = decltype(element);
+      constexpr int U = decltype(width)::value;
+      B200MOE_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(sort_few_kernel<T_, U>), kMostHist));
+      B200MOE_CUDA_OK(launch_overlapped(sort_few_kernel<T_, U>, dim3(T), kSortThreads, (kSortWarps + 1) * E * sizeof(int),
+                                        static_cast<cudaStream_t>(stream), s, a, static_cast<const T_*>(hidden), pitch,
+                                        expert_offsets, row_of_pair, static_cast<T_*>(rows)));
+      B200MOE_LAUNCH_OK("sort_few_kernel");
+      return B200MOE_OK;
+    });
+  }
+  rc = b200moe_sort_pairs(expert_index, index_bytes, T, K, E, expert_offsets, row_of_pair, workspace, workspace_bytes, stream);
   return rc != B200MOE_OK ? rc : b200moe_sort_rows(hidden, dtype, pitch, T, K, H, E, row_of_pair, expert_offsets, rows, stream);
 }
 

@@ -127,6 +127,25 @@ def test_rows_there_and_back(T, K, E, H, dropped, repeat, dtype):
     assert torch.equal(ones, want)
 
 
+@pytest.mark.parametrize("T,K,E", [(1, 1, 1), (1, 1, 1024), (16, 8, 128), (128, 16, 1024), (127, 16, 3), (129, 8, 256), (128, 17, 64),
+                                   (40, 51, 7), (100, 20, 9)])
+@pytest.mark.parametrize("H", [8, 4096, 4097, 9002])
+def test_rows_of_few_tokens(T, K, E, H):
+    """Order and rows of a few tokens come from one launch, which agrees with the two that more tokens take."""
+    import nki_library_b200 as m
+    idx = _ids(T, K, E, T + K + E, 0.2, True)
+    hidden = torch.randn((T, H), device="cuda", generator=_gen(T)).bfloat16()
+    rows, plan = m.moe_sort_tokens(hidden, idx, E)
+    offsets, row = ref.sorted_rows(idx, E)
+    assert torch.equal(plan.expert_offsets.cpu(), offsets) and torch.equal(plan.row_of_pair.cpu(), row)
+    alone = m.moe_sort_plan(idx, E)
+    assert all(torch.equal(a, b) for a, b in zip(alone[:2], plan[:2]))
+    want = torch.zeros((T * K, H), dtype=torch.bfloat16, device="cuda")
+    live = row >= 0
+    want[row[live].long().cuda()] = hidden[torch.arange(T)[:, None].expand(T, K)[live].cuda()]
+    assert torch.equal(rows, want)
+
+
 def test_rows_with_other_strides():
     import nki_library_b200 as m
     gen = _gen(3)
