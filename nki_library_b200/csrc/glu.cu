@@ -22,44 +22,69 @@ __device__ __forceinline__ float rcp(float x) {
   return r;
 }
 
-// act(g) and act'(g) in fp32.  SiLU, Swish and the tanh form of GELU are g sigma(z(g)): act' = sigma + g sigma (1 - sigma) z'.
-// The two approximations are good to 2^-22 each.
+// Two fp32 operations in one instruction, each rounded as the single ones are.
+__device__ __forceinline__ unsigned long long& bits2(float2& v) { return reinterpret_cast<unsigned long long&>(v); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(bits2(r)) : "l"(bits2(a)), "l"(bits2(b)));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(bits2(r)) : "l"(bits2(a)), "l"(bits2(b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(bits2(r)) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// act(g) and act'(g) of two values in fp32.  SiLU, Swish and the tanh form of GELU are g sigma(z(g)): act' = sigma + g sigma
+// (1 - sigma) z'.  The two approximations are good to 2^-22 each.
 template <int ACT>
-__device__ __forceinline__ void act_and_slope(float g, float& act, float& slope) {
+__device__ __forceinline__ void act_and_slope(float2 g, float2& act, float2& slope) {
   constexpr float kLog2e = 1.4426950408889634f;
   if constexpr (ACT == B200MOE_ACT_GELU) {
     // With a = |g| / sqrt 2 and t = 1 / (1 + 0.51 a): erfc(a) exp(a^2) = t Q(t), a least-squares fit of the relative error over
     // a in [0, 10] that is off by 1.2e-6 of itself; the exponential is what the slope needs too.  The tail keeps its relative
-    // precision.  (65536 x 4096 with checkpoint: 371 us; with erfcf, exp and a division from the library 856.)
-    const float e = ex2(-0.5f * kLog2e * g * g);
-    const float t = rcp(fmaf(0.51f * 0.70710678118654752f, fabsf(g), 1.0f));
-    float q = 9.450306e-2f;
-    q = fmaf(q, t, -3.5914552e-1f);
-    q = fmaf(q, t, 3.5846028e-1f);
-    q = fmaf(q, t, 5.5042729e-2f);
-    q = fmaf(q, t, 2.7906981e-1f);
-    q = fmaf(q, t, 2.8415164e-1f);
-    q = fmaf(q, t, 2.8791755e-1f);
-    const float tail = 0.5f * q * t * e;
-    const float cdf = g < 0.0f ? tail : 1.0f - tail;
-    act = g * cdf;
-    slope = fmaf(g * 0.39894228040143268f, e, cdf);
+    // precision.  (65536 x 4096 with checkpoint: 353 us; with erfcf, exp and a division from the library 856.)  Here Q / 2.
+    const float2 square = mul2(mul2(g, both(-0.5f * kLog2e)), g);
+    const float2 e = make_float2(ex2(square.x), ex2(square.y));
+    const float2 d = fma2(both(0.51f * 0.70710678118654752f), make_float2(fabsf(g.x), fabsf(g.y)), both(1.0f));
+    const float2 t = make_float2(rcp(d.x), rcp(d.y));
+    float2 q = both(4.725153e-2f);
+    q = fma2(q, t, both(-1.7957276e-1f));
+    q = fma2(q, t, both(1.7923014e-1f));
+    q = fma2(q, t, both(2.75213645e-2f));
+    q = fma2(q, t, both(1.39534905e-1f));
+    q = fma2(q, t, both(1.4207582e-1f));
+    q = fma2(q, t, both(1.43958775e-1f));
+    const float2 tail = mul2(mul2(q, t), e);
+    const float2 rest = fma2(tail, both(-1.0f), both(1.0f));
+    const float2 cdf = make_float2(g.x < 0.0f ? tail.x : rest.x, g.y < 0.0f ? tail.y : rest.y);
+    act = mul2(g, cdf);
+    slope = fma2(mul2(g, both(0.39894228040143268f)), e, cdf);
   } else {
-    float z, dz;  // z in powers of two
+    float2 z, dz;  // z in powers of two
     if constexpr (ACT == B200MOE_ACT_SILU) {
-      z = kLog2e * g;
-      dz = 1.0f;
+      z = mul2(both(-kLog2e), g);
+      dz = both(1.0f);
     } else if constexpr (ACT == B200MOE_ACT_SWISH) {
-      z = 1.702f * kLog2e * g;
-      dz = 1.702f;
+      z = mul2(both(-1.702f * kLog2e), g);
+      dz = both(1.702f);
     } else {  // (1 + tanh(z / 2)) / 2 = sigma(z)
-      const float g2 = fminf(g * g, 1e30f);  // keeps dz finite
-      z = 1.5957691216057308f * kLog2e * g * fmaf(0.044715f, g2, 1.0f);
-      dz = 1.5957691216057308f * fmaf(3.0f * 0.044715f, g2, 1.0f);
+      float2 g2 = mul2(g, g);
+      g2 = make_float2(fminf(g2.x, 1e30f), fminf(g2.y, 1e30f));  // keeps dz finite
+      z = mul2(mul2(both(-1.5957691216057308f * kLog2e), g), fma2(both(0.044715f), g2, both(1.0f)));
+      dz = fma2(both(1.5957691216057308f * 3.0f * 0.044715f), g2, both(1.5957691216057308f));
     }
-    const float sigma = rcp(1.0f + ex2(-z));
-    act = g * sigma;
-    slope = fmaf(act * (1.0f - sigma), dz, sigma);
+    const float2 d = add2(both(1.0f), make_float2(ex2(z.x), ex2(z.y)));
+    const float2 sigma = make_float2(rcp(d.x), rcp(d.y));
+    act = mul2(g, sigma);
+    const float2 turn = mul2(act, fma2(sigma, both(-1.0f), both(1.0f)));
+    slope = fma2(turn, dz, sigma);
   }
 }
 
@@ -82,7 +107,10 @@ __device__ __forceinline__ uint2 keep8(float (&v)[8], uint32_t& scale_byte) {
   // exponent of top / 448 = top / (1.75 * 2^8), rounded up: one more where top's mantissa is above 1.75
   scale_byte = max(static_cast<int>((__float_as_uint(top) + 0x1fffffu) >> 23) - 8, 0);
   const float f = __uint_as_float((254u - scale_byte) << 23);  // 1 / s, a normal number for every s
-  return make_uint2(pack4_e4m3(v[0] * f, v[1] * f, v[2] * f, v[3] * f), pack4_e4m3(v[4] * f, v[5] * f, v[6] * f, v[7] * f));
+  float2 x[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = mul2(make_float2(v[2 * j], v[2 * j + 1]), both(f));
+  return make_uint2(pack4_e4m3(x[0].x, x[0].y, x[1].x, x[1].y), pack4_e4m3(x[2].x, x[2].y, x[3].x, x[3].y));
 }
 
 __device__ __forceinline__ void kept8(uint2 codes, uint32_t scale_byte, float (&v)[8]) {
@@ -92,9 +120,9 @@ __device__ __forceinline__ void kept8(uint2 codes, uint32_t scale_byte, float (&
   for (int i = 0; i < 4; ++i) {
     const __nv_fp8x2_storage_t two = static_cast<__nv_fp8x2_storage_t>(w[i >> 1] >> (16 * (i & 1)));
     const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3));
-    const float2 f = __half22float2(h);
-    v[2 * i] = f.x * scale;
-    v[2 * i + 1] = f.y * scale;
+    const float2 f = mul2(__half22float2(h), both(scale));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
   }
   if (scale_byte >= 247) {  // 256 * 2^120, what the largest finite values round up to, is no fp32 number
 #pragma unroll
@@ -129,8 +157,8 @@ __device__ __forceinline__ Place place(const Shape& s) {
   return {r, c, r < s.rows && c < s.I};
 }
 
-// Bound by the bytes it moves: 65536 x 4096, SiLU, 2.16 GB with the checkpoint in 341 us, 1.61 GB without in 249; GELU 371 (its
-// arithmetic shows beside the checkpoint's) and 244.
+// Bound by the bytes it moves: 65536 x 4096, SiLU, 2.16 GB with the checkpoint in 341 us, 1.61 GB without in 249; GELU 353 and
+// 245 (one value at a time, its arithmetic showed: 391 and 254).
 template <int ACT, bool KEEP>
 __global__ void __launch_bounds__(256) glu_kernel(Shape s, const __nv_bfloat16* gate_up, int64_t pitch, __nv_bfloat16* m,
                                                   uint8_t* codes, uint8_t* scales) {
@@ -155,10 +183,12 @@ __global__ void __launch_bounds__(256) glu_kernel(Shape s, const __nv_bfloat16* 
       unpack8_bf16(raw[i][0], g);
       unpack8_bf16(raw[i][1], u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float a, slope;
-        act_and_slope<ACT>(g[j], a, slope);
-        out[j] = a * u[j];
+      for (int j = 0; j < 8; j += 2) {
+        float2 a, slope;
+        act_and_slope<ACT>(make_float2(g[j], g[j + 1]), a, slope);
+        const float2 v = mul2(a, make_float2(u[j], u[j + 1]));
+        out[j] = v.x;
+        out[j + 1] = v.y;
       }
       if (inside[i]) *reinterpret_cast<uint4*>(m + row * s.I + at.c) = pack8_bf16(out);
       if constexpr (KEEP) {
@@ -177,9 +207,10 @@ __global__ void __launch_bounds__(256) glu_kernel(Shape s, const __nv_bfloat16* 
   }
 }
 
-// The same 2.16 GB in 340 us, 2.70 GB with m in 430; GELU 399 and 455.
+// The same 2.16 GB in 343 us, 2.70 GB with m in 435; GELU 412 and 441.  Four CTAs per SM: with 66 to 74 registers, three, it took
+// 370 and 435, with five and 51 registers 381 and 459.
 template <int ACT>
-__global__ void __launch_bounds__(256) glu_backward_kernel(Shape s, const __nv_bfloat16* d_m, int64_t pitch, const uint8_t* codes,
+__global__ void __launch_bounds__(256, 4) glu_backward_kernel(Shape s, const __nv_bfloat16* d_m, int64_t pitch, const uint8_t* codes,
                                                            const uint8_t* scales, __nv_bfloat16* d_gate_up, __nv_bfloat16* m) {
   grid_enter(d_m, codes, scales);
   const Place at = place(s);
@@ -208,12 +239,17 @@ __global__ void __launch_bounds__(256) glu_backward_kernel(Shape s, const __nv_b
       kept8(cg[i], sg[i], g);
       kept8(cu[i], su[i], u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float a, slope;
-        act_and_slope<ACT>(g[j], a, slope);
-        out[j] = a * u[j];
-        dg[j] = d[j] * u[j] * slope;
-        du[j] = d[j] * a;
+      for (int j = 0; j < 8; j += 2) {
+        const float2 up = make_float2(u[j], u[j + 1]), dm = make_float2(d[j], d[j + 1]);
+        float2 a, slope;
+        act_and_slope<ACT>(make_float2(g[j], g[j + 1]), a, slope);
+        const float2 v = mul2(a, up), vg = mul2(mul2(dm, up), slope), vu = mul2(dm, a);
+        out[j] = v.x;
+        out[j + 1] = v.y;
+        dg[j] = vg.x;
+        dg[j + 1] = vg.y;
+        du[j] = vu.x;
+        du[j + 1] = vu.y;
       }
       if (d_gate_up != nullptr) {
         *reinterpret_cast<uint4*>(d_gate_up + row * 2 * s.I + at.c) = pack8_bf16(dg);
