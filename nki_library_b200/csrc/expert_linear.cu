@@ -18,6 +18,7 @@
 // Warps of a persistent CTA (256 threads, weight grad 416):
 //   0, 3   TMA producers of the column and the row operand
 //   1      allocates TMEM; in the even CTA issues the MMAs (M 256, K 16), in the odd one hands out the pair's tiles
+//   2      product: clears the rows of no expert
 //   last   weight grad: fetches the rows of a contraction that do not fill a step of 16 into a buffer of their own, where
 //   2      clears those behind them, which belong to the next expert (or hold what a caller left behind the last one), so
 //          that they add nothing, whatever they hold.  (One warp for both waits out each copy before it asks for the next:
@@ -478,6 +479,16 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
       }
     }
     __syncwarp();
+  } else if (!WGRAD && warp == 2) {
+    // ------------------------------------------------------------ rows of no expert, beside the tiles
+    if (p.parts == 1) {
+      const int lo = s.first[0], hi = s.first[p.E], none = lo + p.R - hi;
+      for (int i = blockIdx.x; i < none; i += gridDim.x) {
+        uint4* row = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(i < lo ? i : i - lo + hi) * p.cols);
+#pragma unroll 8
+        for (int c = lane; c < p.cols >> 3; c += 32) row[c] = make_uint4(0, 0, 0, 0);
+      }
+    }
   } else if (WGRAD && warp == 2) {
     if constexpr (WGRAD) {
     // ------------------------------------------------------------ ragged ends
@@ -526,14 +537,6 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3, group = (warp - 4) >> 2;
     int it = 0;
-    if (!WGRAD && p.parts == 1) {
-      // rows of no expert
-      const int lo = s.first[0], hi = s.first[p.E], none = lo + p.R - hi;
-      for (int i = blockIdx.x * 4 * kGroups + warp - 4; i < none; i += gridDim.x * 4 * kGroups) {
-        uint4* row = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(i < lo ? i : i - lo + hi) * p.cols);
-        for (int c = lane; c < p.cols >> 3; c += 32) row[c] = make_uint4(0, 0, 0, 0);
-      }
-    }
     for (int tile = walk.next(); tile >= 0; tile = walk.next()) {
       const Tile t = decode_tile<WGRAD>(p, s, tile);
       const int64_t row0 = (WGRAD ? static_cast<int64_t>(t.expert) * p.rows : 0) + t.row0;
@@ -761,7 +764,7 @@ extern "C" int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch,
   // the queue cost 4 to 9 us (64 experts of 2048 x 2048, 125 rows each: 109 us without, 118 with; 9216 rows on 6 experts of
   // 64 x 13376: 64 and 73, of 4096 x 4096 211 and 215); so they do for the weight gradient's short contractions (4 x 1024
   // rows, 4096 x 14336: 353 and 367 us).
-  const int64_t bytes = 2 * (static_cast<int64_t>(E) * D0 * D1 + static_cast<int64_t>(R) * (static_cast<int64_t>(D0) + D1));
+  const int64_t bytes = 2 * (static_cast<int64_t>(E) * D0 * D1 + static_cast<int64_t>(R) * k);
   if (R >= 512 * static_cast<int64_t>(E) && bytes >= (int64_t{1} << 29) && most_tiles >= 4 * (sm_count() / 2)) {
     p.taken = status + 1;
     p.queue = k >= 1024 ? 2 : kQueue;
