@@ -7,7 +7,7 @@ from typing import Optional, Tuple
 import torch
 
 from .... import _lib
-from .launch import launch, needs_grad, once, pitch_of, refuse, same_device, tile_rows
+from .launch import MOST_ROWS, launch, needs_grad, once, pitch_of, refuse, same_device, tile_rows
 from .sort_tokens import MAX_EXPERTS
 
 
@@ -30,6 +30,7 @@ def _stored(weight: torch.Tensor) -> Tuple[torch.Tensor, bool]:
     return weight.clone(memory_format=torch.contiguous_format), False
 
 
+MOST_COLUMNS = 2 ** 27
 _LONG = 49 * 64  # contractions below this length are never cut into parts, and need no workspace
 
 
@@ -118,8 +119,8 @@ def check_rows_and_weight(rows: torch.Tensor, weight: torch.Tensor, expert_offse
         refuse(f"between 1 and {MAX_EXPERTS} experts, got {E}")
     if expert_offsets.dtype != torch.int32 or expert_offsets.shape != (E + 1,) or not expert_offsets.is_contiguous():
         refuse(f"expert_offsets must be int32 [E + 1] = [{E + 1}]")
-    if R >= 2 ** 31:
-        refuse("at most 2^31 - 1 rows")
+    if R > MOST_ROWS or max(K, N) > MOST_COLUMNS:
+        refuse(f"at most 2^30 rows and matrices of at most 2^27 either way, got {R} rows and {K} x {N}")
 
 
 def expert_linear(rows: torch.Tensor, weight: torch.Tensor, expert_offsets: torch.Tensor,

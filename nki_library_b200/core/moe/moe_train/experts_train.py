@@ -6,7 +6,7 @@ import torch
 
 from .... import _lib
 from ...utils.common_types import ActFnType
-from .expert_linear import check_rows_and_weight, product, weight_grad
+from .expert_linear import MOST_COLUMNS, check_rows_and_weight, product, weight_grad
 from .launch import needs_grad, once, same_device, tile_rows
 from .moe_glu import glu_backward, glu_forward
 from .sort_tokens import moe_sort_tokens, moe_unsort_tokens
@@ -46,14 +46,15 @@ def moe_expert_mlp(rows: torch.Tensor, gate_up_proj_weight: torch.Tensor, down_p
     same_device(rows, gate_up_proj_weight, down_proj_weight, expert_offsets)
     A = _lib.kernel_assert
     if gate_up_proj_weight.dim() == 4:
+        A(gate_up_proj_weight.shape[2] == 2, "gate_up_proj_weight must be [E, H, 2, I] or [E, H, 2 I]")
         gate_up_proj_weight = gate_up_proj_weight.flatten(2)
     check_rows_and_weight(rows, gate_up_proj_weight, expert_offsets, "gate_up_proj_weight")
     A(isinstance(activation_function, ActFnType), "activation_function must be an ActFnType")
     A(down_proj_weight.dim() == 3 and down_proj_weight.dtype == torch.bfloat16 and
       down_proj_weight.shape[0] == gate_up_proj_weight.shape[0] and
       2 * down_proj_weight.shape[1] == gate_up_proj_weight.shape[2], "down_proj_weight must be bfloat16 [E, I, H_out]")
-    A(down_proj_weight.shape[1] % 8 == 0 and down_proj_weight.shape[2] % 8 == 0 and down_proj_weight.shape[2] > 0,
-      "both sizes of down_proj_weight's matrices must be multiples of 8")
+    A(down_proj_weight.shape[1] % 8 == 0 and down_proj_weight.shape[2] % 8 == 0 and
+      0 < down_proj_weight.shape[2] <= MOST_COLUMNS, "both sizes of down_proj_weight's matrices must be multiples of 8, at most 2^27")
     act = activation_function.value
     if needs_grad(rows, gate_up_proj_weight, down_proj_weight):
         return _ExpertMLP.apply(rows, gate_up_proj_weight, down_proj_weight, expert_offsets, act)

@@ -10,6 +10,8 @@ import torch
 
 from .... import _lib
 
+MOST_ROWS = 2 ** 30  # of a product or an activation: indices of tiles behind the last row stay below 2^31
+
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 

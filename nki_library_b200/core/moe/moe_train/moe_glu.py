@@ -8,7 +8,9 @@ import torch
 
 from .... import _lib
 from ...utils.common_types import ActFnType
-from .launch import launch, needs_grad, once, pitch_of, refuse, tile_rows
+from .launch import MOST_ROWS, launch, needs_grad, once, pitch_of, refuse, tile_rows
+
+_MOST_I = 2 ** 26
 
 
 def glu_forward(gate_up: torch.Tensor, act: int, keep: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
@@ -24,11 +26,6 @@ def glu_forward(gate_up: torch.Tensor, act: int, keep: bool) -> Tuple[torch.Tens
         launch(device, "b200moe_glu", gate_up.data_ptr(), pitch_of(gate_up), R, I, act, m.data_ptr(), codes,
                codes + R * two_I if keep else None)
     return m, kept
-
-
-def kept_parts(kept: torch.Tensor, R: int, I: int) -> Tuple[torch.Tensor, torch.Tensor]:
-    """The codes ``[R, 2 I]`` and scales ``[R, 2, ceil(I / 32)]`` of a checkpoint."""
-    return kept[:R * 2 * I].view(R, 2 * I), kept[R * 2 * I:].view(R, 2, (I + 31) // 32)
 
 
 def glu_backward(d_m: Optional[torch.Tensor], kept: torch.Tensor, R: int, I: int, act: int,
@@ -81,6 +78,8 @@ def moe_glu(gate_up: torch.Tensor, activation_function: ActFnType = ActFnType.Si
         refuse("activation_function must be an ActFnType")
     if gate_up.shape[1] == 0 or gate_up.shape[1] % 16:
         refuse(f"I must be a multiple of 8, gate_up has {gate_up.shape[1]} columns")
+    if gate_up.shape[0] > MOST_ROWS or gate_up.shape[1] > 2 * _MOST_I:
+        refuse(f"at most 2^30 rows of at most 2^27 columns, got {list(gate_up.shape)}")
     if needs_grad(gate_up):
         return _Glu.apply(gate_up, activation_function.value)
     return glu_forward(gate_up, activation_function.value, False)[0]

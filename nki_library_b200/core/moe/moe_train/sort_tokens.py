@@ -11,6 +11,7 @@ from .launch import launch, needs_grad, once, pitch_of, refuse, same_device, uni
 
 MAX_EXPERTS = 1024
 _ID_TYPES = (torch.int32, torch.uint32, torch.int64)
+_MOST_COLUMNS = 2 ** 30
 _ONE_LAUNCH = 2048  # pairs that the sort takes without a workspace
 
 
@@ -84,6 +85,8 @@ def _check_plan(plan: SortedTokens) -> Tuple[int, int]:
 def _check_rows(t: torch.Tensor, name: str) -> None:
     if t.dim() != 2 or t.dtype not in (torch.bfloat16, torch.float32):
         refuse(f"{name} must be 2-D, bfloat16 or float32")
+    if t.shape[1] > _MOST_COLUMNS:
+        refuse(f"{name} must have at most 2^30 columns")
 
 
 def _unsort_rows(rows: torch.Tensor, affinities: Optional[torch.Tensor], row_of_pair: torch.Tensor) -> torch.Tensor:

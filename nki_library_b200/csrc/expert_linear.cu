@@ -39,6 +39,8 @@ namespace b200moe {
 namespace {
 
 constexpr int kMaxExperts = 1024;
+constexpr int kMaxRows = 1 << 30;  // indices of tiles behind the last row stay below 2^31
+constexpr int kMaxSize = 1 << 27;  // of a matrix; fewer than 2^20 column tiles
 constexpr int kStages = 6;
 constexpr int kOperand = 128 * 128;  // bytes of one operand's part of a stage: 128 rows of 128 bytes
 constexpr int kStage = 2 * kOperand;
@@ -722,10 +724,10 @@ extern "C" int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch,
                                       b200moe_stream_t stream) {
   B200MOE_REQUIRE(rows_bf16 && weight_bf16 && expert_offsets && out_bf16 && status, B200MOE_ERR_INVALID,
                   "expert_product: null pointer argument");
-  B200MOE_REQUIRE(R > 0 && E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID,
-                  "expert_product: need at least one row and between 1 and %d experts", kMaxExperts);
-  B200MOE_REQUIRE(D0 > 0 && D1 > 0 && D0 % 8 == 0 && D1 % 8 == 0, B200MOE_ERR_INVALID,
-                  "expert_product: both sizes of a weight matrix must be positive multiples of 8, got %d x %d", D0, D1);
+  B200MOE_REQUIRE(R > 0 && R <= kMaxRows && E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID,
+                  "expert_product: need at least one row and at most 2^30, and between 1 and %d experts", kMaxExperts);
+  B200MOE_REQUIRE(D0 > 0 && D1 > 0 && D0 % 8 == 0 && D1 % 8 == 0 && D0 <= kMaxSize && D1 <= kMaxSize, B200MOE_ERR_INVALID,
+                  "expert_product: both sizes of a weight matrix must be positive multiples of 8, at most 2^27, got %d x %d", D0, D1);
   const int k = contract_last ? D1 : D0, n = contract_last ? D0 : D1;
   B200MOE_REQUIRE(rows_ok(rows_bf16, rows_pitch, k) && rows_ok(weight_bf16, w_pitch, D1) &&
                       rows_ok(weight_bf16, w_expert_pitch, D1),
@@ -739,7 +741,6 @@ extern "C" int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch,
   p.cols = n;
   p.k = k;
   p.col_tiles = (n + 255) / 256;
-  B200MOE_REQUIRE(p.col_tiles < (1 << 20), B200MOE_ERR_INVALID, "expert_product: too many output columns");
   p.per_matrix = p.per_group = make_divisor(static_cast<uint32_t>(kGroup * p.col_tiles));
   p.out = static_cast<__nv_bfloat16*>(out_bf16);
   p.status = status;
@@ -782,10 +783,10 @@ extern "C" int b200moe_expert_weight_grad(const void* a_bf16, int64_t a_pitch, c
                                           void* workspace, size_t workspace_bytes, int32_t* status, b200moe_stream_t stream) {
   B200MOE_REQUIRE(a_bf16 && b_bf16 && expert_offsets && out_bf16 && status, B200MOE_ERR_INVALID,
                   "expert_weight_grad: null pointer argument");
-  B200MOE_REQUIRE(R > 0 && E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID,
-                  "expert_weight_grad: need at least one row and between 1 and %d experts", kMaxExperts);
-  B200MOE_REQUIRE(M > 0 && N > 0 && M % 8 == 0 && N % 8 == 0, B200MOE_ERR_INVALID,
-                  "expert_weight_grad: both sizes of a weight matrix must be positive multiples of 8, got %d x %d", M, N);
+  B200MOE_REQUIRE(R > 0 && R <= kMaxRows && E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID,
+                  "expert_weight_grad: need at least one row and at most 2^30, and between 1 and %d experts", kMaxExperts);
+  B200MOE_REQUIRE(M > 0 && N > 0 && M % 8 == 0 && N % 8 == 0 && M <= kMaxSize && N <= kMaxSize, B200MOE_ERR_INVALID,
+                  "expert_weight_grad: both sizes of a weight matrix must be positive multiples of 8, at most 2^27, got %d x %d", M, N);
   B200MOE_REQUIRE(rows_ok(a_bf16, a_pitch, M) && rows_ok(b_bf16, b_pitch, N), B200MOE_ERR_INVALID,
                   "expert_weight_grad: rows must start on 16-byte boundaries");
   B200MOE_REQUIRE((reinterpret_cast<uintptr_t>(out_bf16) & 15) == 0, B200MOE_ERR_INVALID,
@@ -807,7 +808,6 @@ extern "C" int b200moe_expert_weight_grad(const void* a_bf16, int64_t a_pitch, c
   B200MOE_REQUIRE(p.parts == 1 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
                                    workspace_bytes >= b200moe_expert_weight_grad_workspace_bytes(R, E, M, N)),
                   B200MOE_ERR_WORKSPACE, "expert_weight_grad: workspace too small or not 16-byte aligned");
-  B200MOE_REQUIRE(p.col_tiles < (1 << 20), B200MOE_ERR_INVALID, "expert_weight_grad: too many output columns");
   B200MOE_REQUIRE(tiles < (int64_t{1} << 30), B200MOE_ERR_INVALID, "expert_weight_grad: too many output tiles");
   p.per_matrix = make_divisor(static_cast<uint32_t>(p.row_tiles * p.col_tiles));
   p.per_group = make_divisor(static_cast<uint32_t>(kGroup * p.col_tiles));

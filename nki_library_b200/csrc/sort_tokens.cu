@@ -52,11 +52,51 @@ __global__ void __launch_bounds__(kSortThreads) count_pairs_kernel(SortArgs a, i
   for (int e = threadIdx.x; e < a.E; e += kSortThreads) chunk_counts[static_cast<int64_t>(blockIdx.x) * a.E + e] = hist[e];
 }
 
+// The chunks' counts turned into sums over all chunks up to and with each: eight experts per CTA, a 128th of the chunks per
+// thread.  Without it every CTA adds all chunks' counts up, whose time grows with their square; with it there is a third launch.
+// Without / with, order of 8 x T pairs: T 32768 and 128 experts 26.6 / 30.6 us, 1024 experts 51 / 31; T 131072 and 8 experts 22.0 /
+// 23.6, 128 44.5 / 25.1; T 1048576 and 64 experts 761 / 111.
+bool scan_pays(int64_t chunks, int E) { return chunks * (E > 32 ? E : 32) > 32768; }
+constexpr int kScanExperts = 8;
+constexpr int kScanParts = 128;
+__global__ void __launch_bounds__(kScanExperts * kScanParts) scan_counts_kernel(int* chunk_counts, int chunks, int E) {
+  __shared__ int s_warp[kScanParts / 4][kScanExperts];
+  grid_enter(chunk_counts);
+  const int column = threadIdx.x % kScanExperts, part = threadIdx.x / kScanExperts;
+  const int e = blockIdx.x * kScanExperts + column, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (chunks + kScanParts - 1) / kScanParts;
+  const int c0 = min(part * per, chunks), c1 = e < E ? min(c0 + per, chunks) : c0;
+  int* counts = chunk_counts + e;
+  int sum = 0;
+#pragma unroll 16
+  for (int c = c0; c < c1; ++c) sum += counts[static_cast<int64_t>(c) * E];
+  int scan = sum;  // of a warp's four parts
+#pragma unroll
+  for (int o = kScanExperts; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += u;
+  }
+  if (lane >= 32 - kScanExperts) s_warp[warp][column] = scan;
+  __syncthreads();
+  int run = scan - sum;
+  for (int w = 0; w < warp; ++w) run += s_warp[w][column];
+  for (int c = c0; c < c1; c += 16) {
+    int n[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) n[i] = c + i < c1 ? counts[static_cast<int64_t>(c + i) * E] : 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      run += n[i];
+      if (c + i < c1) counts[static_cast<int64_t>(c + i) * E] = run;
+    }
+  }
+}
+
 // Rows of one chunk's pairs, by a whole CTA; `put(pair, row)` is called once per pair, -1 for none.  Every CTA adds the chunks'
-// counts up for itself: its own base per expert costs no third launch.  Returns the number of rows; `offsets` may be NULL.
+// counts up for itself, unless they are `scanned`.  Returns the number of rows; `offsets` may be NULL.
 template <typename Put>
-__device__ __forceinline__ int order_chunk(const SortArgs& a, int chunk, int chunks, const int* chunk_counts, int* hist,
-                                           int32_t* offsets, const Put& put) {
+__device__ __forceinline__ int order_chunk(const SortArgs& a, int chunk, int chunks, const int* chunk_counts, bool scanned,
+                                           int* hist, int32_t* offsets, const Put& put) {
   __shared__ int s_warp[kSortWarps], s_before[kSortThreads], s_total[kSortThreads];
   int* base = hist + kSortWarps * a.E;  // hist [kSortWarps][E], then base [E]
   const int64_t p0 = static_cast<int64_t>(chunk) * kChunk;
@@ -78,7 +118,7 @@ __device__ __forceinline__ int order_chunk(const SortArgs& a, int chunk, int chu
   __syncthreads();
   // `width` experts at a time, every `parts`-th chunk per thread: one memory latency for each of a thread's chunks would be the
   // whole launch (262144 pairs, 128 experts, a thread per expert: 31 us, 15 so)
-  int run = 0;  // rows of the experts before this round's
+  int run = 0;  // rows of the experts before e0
   const int width = min(kSortThreads, max(32, 1 << (32 - __clz(a.E - 1)))), parts = kSortThreads / width;
   const int part = threadIdx.x / width, column = threadIdx.x - part * width;
   for (int e0 = 0; e0 < a.E; e0 += width) {
@@ -90,6 +130,11 @@ __device__ __forceinline__ int order_chunk(const SortArgs& a, int chunk, int chu
 #pragma unroll
           for (int w = 0; w < kSortWarps; ++w) total += hist[w * a.E + e];
         }
+      } else if (scanned) {
+        if (part == 0) {
+          before = chunk > 0 ? chunk_counts[static_cast<int64_t>(chunk - 1) * a.E + e] : 0;
+          total = chunk_counts[static_cast<int64_t>(chunks - 1) * a.E + e];
+        }
       } else {
 #pragma unroll 16
         for (int c = part; c < chunks; c += parts) {
@@ -99,7 +144,7 @@ __device__ __forceinline__ int order_chunk(const SortArgs& a, int chunk, int chu
         }
       }
     }
-    if (parts > 1 && chunks > 1) {
+    if (parts > 1 && chunks > 1 && !scanned) {
       s_before[threadIdx.x] = before;
       s_total[threadIdx.x] = total;
       __syncthreads();
@@ -157,11 +202,11 @@ __device__ __forceinline__ int order_chunk(const SortArgs& a, int chunk, int chu
   return run;
 }
 
-__global__ void __launch_bounds__(kSortThreads) place_pairs_kernel(SortArgs a, const int* chunk_counts, int32_t* offsets,
-                                                                   int32_t* row_of_pair) {
+__global__ void __launch_bounds__(kSortThreads) place_pairs_kernel(SortArgs a, const int* chunk_counts, bool scanned,
+                                                                   int32_t* offsets, int32_t* row_of_pair) {
   extern __shared__ int hist[];
   grid_enter(a.index, chunk_counts);
-  order_chunk(a, blockIdx.x, gridDim.x, chunk_counts, hist, blockIdx.x == 0 ? offsets : nullptr,
+  order_chunk(a, blockIdx.x, gridDim.x, chunk_counts, scanned, hist, blockIdx.x == 0 ? offsets : nullptr,
               [&](int64_t p, int row) { row_of_pair[p] = row; });
 }
 
@@ -296,7 +341,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_few_kernel(SortArgs s, RowA
   const int64_t t = blockIdx.x;
   P piece;  // on its way while the order is worked out
   piece.fetch(hidden + t * pitch, 0, a.H);
-  const int used = order_chunk(s, 0, 1, nullptr, hist, first ? offsets : nullptr, [&](int64_t p, int row) {
+  const int used = order_chunk(s, 0, 1, nullptr, false, hist, first ? offsets : nullptr, [&](int64_t p, int row) {
     s_row[p] = row;
     if (first) row_of_pair[p] = row;
   });
@@ -449,8 +494,8 @@ Layout row_layout(int T, int H, int per_thread, int threads, bool spread) {
 
 int check_rows(const char* name, int dtype, int T, int K, int H, int64_t pitch) {
   B200MOE_REQUIRE(dtype == B200MOE_F32 || dtype == B200MOE_BF16, B200MOE_ERR_INVALID, "%s: rows must be fp32 or bf16", name);
-  B200MOE_REQUIRE(T > 0 && K > 0 && H > 0 && static_cast<int64_t>(T) * K <= INT32_MAX, B200MOE_ERR_INVALID,
-                  "%s: need T, K, H > 0 and at most 2^31 - 1 pairs", name);
+  B200MOE_REQUIRE(T > 0 && K > 0 && H > 0 && H <= (1 << 30) && static_cast<int64_t>(T) * K <= INT32_MAX, B200MOE_ERR_INVALID,
+                  "%s: need T, K, H > 0, at most 2^31 - 1 pairs and 2^30 columns", name);
   B200MOE_REQUIRE(pitch >= 0, B200MOE_ERR_INVALID, "%s: negative row pitch", name);
   return B200MOE_OK;
 }
@@ -500,9 +545,15 @@ extern "C" int b200moe_sort_pairs(const void* expert_index, int index_bytes, int
     B200MOE_CUDA_OK(launch_overlapped(count_pairs_kernel, grid, kSortThreads, E * sizeof(int), st, a, static_cast<int*>(workspace)));
     B200MOE_LAUNCH_OK("count_pairs_kernel");
   }
+  const bool scanned = scan_pays(chunks, E);
+  if (scanned) {
+    B200MOE_CUDA_OK(launch_overlapped(scan_counts_kernel, dim3((E + kScanExperts - 1) / kScanExperts), kScanExperts * kScanParts, 0, st,
+                                      static_cast<int*>(workspace), static_cast<int>(chunks), E));
+    B200MOE_LAUNCH_OK("scan_counts_kernel");
+  }
   B200MOE_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(place_pairs_kernel), kMostHist));
   B200MOE_CUDA_OK(launch_overlapped(place_pairs_kernel, grid, kSortThreads, hist, st, a,
-                                    static_cast<const int*>(workspace), expert_offsets, row_of_pair));
+                                    static_cast<const int*>(workspace), scanned, expert_offsets, row_of_pair));
   B200MOE_LAUNCH_OK("place_pairs_kernel");
   return B200MOE_OK;
 }

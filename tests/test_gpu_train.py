@@ -55,6 +55,23 @@ def test_order(T, K, E, dropped, repeat, dtype):
     assert plan.num_experts == E
 
 
+@pytest.mark.parametrize("T,K,E", [(8192, 8, 1024), (8449, 8, 1024), (70000, 8, 120), (524288, 4, 3), (700001, 3, 9), (1 << 20, 8, 33)])
+def test_order_of_many_pairs(T, K, E):
+    """Either side of the size from which the counts are added up in a launch of their own."""
+    import nki_library_b200 as m
+    idx = torch.randint(-1, E + 1, (T, K), device="cuda", generator=_gen(T), dtype=torch.int32)
+    plan = m.moe_sort_plan(idx, E)
+    flat = idx.flatten().long()
+    none = (flat < 0) | (flat >= E)
+    order = torch.sort(torch.where(none, E, flat), stable=True).indices
+    row = torch.empty_like(order)
+    row[order] = torch.arange(T * K, device="cuda")
+    row[none] = -1
+    assert torch.equal(plan.row_of_pair.flatten().long(), row)
+    counts = torch.bincount(flat[~none], minlength=E)
+    assert plan.expert_offsets.tolist() == [0] + counts.cumsum(0).tolist()
+
+
 def test_order_of_unsigned_strided_and_no_ids():
     import nki_library_b200 as m
     idx = _ids(50, 4, 16, 1)
@@ -394,7 +411,7 @@ def test_activation_and_gradient(R, I, act):
 @pytest.mark.parametrize("I", [8, 32, 104, 2048])
 def test_checkpoint_is_exact(I):
     """Codes and scales bit for bit: magnitudes from the smallest to the largest, ties, blocks of zeros, NaN and infinity."""
-    from nki_library_b200.core.moe.moe_train.moe_glu import glu_backward, glu_forward, kept_parts
+    from nki_library_b200.core.moe.moe_train.moe_glu import glu_backward, glu_forward
     R = 96
     gen = _gen(I)
     x = torch.randn((R, 2 * I), device="cuda", generator=gen) * torch.exp2(
@@ -409,7 +426,7 @@ def test_checkpoint_is_exact(I):
     x[15] = 2.0 ** -133
     x = x.bfloat16()
     _, checkpoint = glu_forward(x, 0, True)
-    codes, scales = kept_parts(checkpoint, R, I)
+    codes, scales = checkpoint[:R * 2 * I].view(R, 2 * I), checkpoint[R * 2 * I:].view(R, 2, (I + 31) // 32)
     e, g, u = _kept_reference(x)
     assert torch.equal(scales.long() - 127, e)
     s = ref.power_of_two(e).repeat_interleave(32, 2)[:, :, :I].reshape(R, 2 * I)
@@ -729,6 +746,33 @@ def test_refusals(call):
         "glu columns": (lambda: m.moe_glu(rows[:, :24]), "multiple of 8"),
         "act": (lambda: m.moe_glu(rows, 0), "ActFnType"),
         "down": (lambda: m.moe_expert_mlp(rows, w1, w2[:, :88], off), "down_proj_weight"),
+    }
+    fn, message = calls[call]
+    with pytest.raises(AssertionError, match=message):
+        fn()
+
+
+@pytest.mark.parametrize("call", ["sort columns", "unsort columns", "rows", "contraction", "columns", "glu rows", "glu columns",
+                                  "four sizes"])
+def test_sizes_that_no_index_holds_are_refused(call):
+    """Sizes beyond the kernels' 32-bit indices, as views of one element: nothing of that size is allocated."""
+    import nki_library_b200 as m
+    one = torch.zeros(1, dtype=torch.bfloat16, device="cuda")
+    idx = torch.zeros((1, 1), dtype=torch.int32, device="cuda")
+    plan = m.moe_sort_plan(idx, 1)
+    off = plan.expert_offsets
+    many, few = 2 ** 32 + 8, torch.zeros((1, 8, 8), dtype=torch.bfloat16, device="cuda")
+    rows = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
+    calls = {
+        "sort columns": (lambda: m.moe_sort_tokens(one.expand(1, many), idx, 1), "columns"),
+        "unsort columns": (lambda: m.moe_unsort_tokens(one.expand(1, many), None, plan), "columns"),
+        "rows": (lambda: m.expert_linear(one.expand(2 ** 30 + 1, 8), few, off), "2\\^30 rows"),
+        "contraction": (lambda: m.expert_linear(one.expand(1, many), one.expand(1, many, 8), off), "2\\^27"),
+        "columns": (lambda: m.expert_linear(one.expand(1, 8), one.expand(1, 8, many), off), "2\\^27"),
+        "glu rows": (lambda: m.moe_glu(one.expand(2 ** 30 + 1, 16)), "2\\^30 rows"),
+        "glu columns": (lambda: m.moe_glu(one.expand(1, 2 * many)), "2\\^27 columns"),
+        "four sizes": (lambda: m.moe_expert_mlp(rows, torch.zeros((1, 64, 4, 8), dtype=torch.bfloat16, device="cuda"),
+                                                torch.zeros((1, 16, 64), dtype=torch.bfloat16, device="cuda"), off), "H, 2, I"),
     }
     fn, message = calls[call]
     with pytest.raises(AssertionError, match=message):
