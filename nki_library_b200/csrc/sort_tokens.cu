@@ -211,73 +211,176 @@ __global__ void __launch_bounds__(kSortThreads) place_pairs_kernel(SortArgs a, c
 }
 
 // ------------------------------------------------------------------ rows
-// The elements of a row that a thread holds at once, `chunk` by `chunk` of the CTA's: one unit of 16 bytes, or, where rows are
-// not made of whole aligned 16 bytes, a few units of 4 or 2 bytes a CTA's width apart.
-template <typename T, int UNIT>
-struct Piece {
-  static constexpr int kUnits = UNIT == 16 ? 1 : 4;  // eight: 252 us for that sum, 804 instead of 317 for its gradients
-  static constexpr int kPer = UNIT / static_cast<int>(sizeof(T));  // elements of a unit
-  static constexpr int kCount = kUnits * kPer;
-  uint32_t raw[UNIT == 16 ? 4 : kUnits];
+// What a thread holds of a row is 16 bytes.
+template <typename T>
+constexpr int kPer = 16 / static_cast<int>(sizeof(T));
 
-  __device__ __forceinline__ static int chunk() { return static_cast<int>(blockDim.x) * kCount; }
-  // Index of the first element of unit u of the chunk that starts at h; units at H and behind do not exist.
-  __device__ __forceinline__ static int index(int h, int u) {
-    return h + (u * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * kPer;
-  }
-  // Only loads, so that a caller's next row is asked for before this one is there (shifting 2-byte units on the spot took 387 us
-  // instead of 187 for the sum of 48000 rows of 5003).
-  __device__ __forceinline__ void fetch(const T* row, int h, int H) {
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& raw, float (&v)[kPer<T>]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      if (index(h, u) >= H) {
-        raw[u] = 0;
-        if constexpr (UNIT == 16) raw[1] = raw[2] = raw[3] = 0;
-        continue;
-      }
-      const T* p = row + index(h, u);
-      if constexpr (UNIT == 16) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-        raw[0] = v.x; raw[1] = v.y; raw[2] = v.z; raw[3] = v.w;
-      } else if constexpr (UNIT == 4) raw[u] = __ldg(reinterpret_cast<const uint32_t*>(p));
-      else raw[u] = __ldg(reinterpret_cast<const uint16_t*>(p));
-    }
-  }
-  // Zero in units that do not exist.
-  __device__ __forceinline__ void values(float (&v)[kCount]) const {
-    if constexpr (sizeof(T) == 2 && UNIT > 2) {
-#pragma unroll
-      for (int i = 0; i < kCount / 2; ++i) {
-        v[2 * i] = __uint_as_float(raw[i] << 16);
-        v[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
-      }
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     } else {
-#pragma unroll
-      for (int i = 0; i < kCount; ++i) v[i] = __uint_as_float(sizeof(T) == 2 ? raw[i] << 16 : raw[i]);
+      v[i] = __uint_as_float(w[i]);
     }
   }
-  __device__ __forceinline__ static void store(T* row, int h, int H, const float (&v)[kCount]) {
-    constexpr int kWords = kCount * static_cast<int>(sizeof(T)) / 4;
-    uint32_t w[kWords > 0 ? kWords : 1];
-    if constexpr (UNIT > 2) {
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float (&v)[kPer<T>]) {
+  uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) {
-        if constexpr (sizeof(T) == 2) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-          w[i] = *reinterpret_cast<const uint32_t*>(&b);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+      w[i] = __float_as_uint(v[i]);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Where a matrix lies: bytes [lo, hi) from its first to its last element; 32 bytes around any element of the rows from `first`
+// on, `count` of them, are still inside.
+struct Span {
+  uintptr_t lo, hi;
+  int first;
+  unsigned count;
+  // Whether `size` bytes at `at`, around an element of the row, are inside.
+  __device__ __forceinline__ bool around(int row, uintptr_t at, int size) const {
+    return static_cast<unsigned>(row - first) < count || (at >= lo && at + size <= hi);
+  }
+};
+
+// The 8 bytes at an aligned address, zero where they lie outside the matrix.  A call, since it is rare: in line it cost the
+// sums 2 to 8 %.
+template <typename T>
+__device__ __noinline__ uint2 careful(uintptr_t at, uintptr_t lo, uintptr_t hi) {
+  if (at >= lo && at + 8 <= hi) return __ldg(reinterpret_cast<const uint2*>(at));
+  unsigned long long w = 0;
+#pragma unroll 1
+  for (int i = 0; i < 8; i += sizeof(T)) {
+    const uintptr_t p = at + i;
+    if (p < lo || p >= hi) continue;
+    if constexpr (sizeof(T) == 2) w |= static_cast<unsigned long long>(__ldg(reinterpret_cast<const uint16_t*>(p))) << (8 * i);
+    else w |= static_cast<unsigned long long>(__ldg(reinterpret_cast<const uint32_t*>(p))) << (8 * i);
+  }
+  return make_uint2(static_cast<uint32_t>(w), static_cast<uint32_t>(w >> 32));
+}
+
+// How a row is cut into pieces of 16 bytes that are aligned where they are stored.  WHOLE: rows are whole aligned 16 bytes
+// everywhere, pieces start at columns 0, kPer, ...  Otherwise pieces are aligned in the row that is written, so that its first
+// and last piece are cut, and a row that lies differently is read as the two or three aligned 8 bytes around each piece.  Sort,
+// sum with weights and its gradients of 16000 tokens x 7163 bf16, top-8: 408, 372, 755 us, and 694, 781, 1157 by 2 bytes at a
+// time; of 6000 x 5004, 8 experts: 112, 105, 203, and 143, 118, 230 by 4 bytes.  (Short rows of whole 4 bytes lose: 100000 x 130,
+// top-8 108, 106, 288 and 68, 141, 204.)
+template <typename T, bool WHOLE>
+struct Cut {
+  // Column of piece p of the row at `row`; pieces with column >= H do not exist.
+  __device__ __forceinline__ static int column(const T* row, int p) {
+    return p * kPer<T> - (WHOLE ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) / static_cast<int>(sizeof(T)));
+  }
+  __device__ __forceinline__ static int pieces(int H) { return (H - 1) / kPer<T> + (WHOLE ? 1 : 2); }
+
+  // kPer elements from any address on.  Only loads, so that a caller's next row is asked for before this one is there.
+  struct Read {
+    uint2 a, b, c;
+    uint32_t m;
+    __device__ __forceinline__ void fetch(const T* first, const Span& span, int row) {
+      if constexpr (WHOLE) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(first));
+        a = make_uint2(v.x, v.y);
+        b = make_uint2(v.z, v.w);
+      } else {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(first);
+        m = static_cast<uint32_t>(at) & 7;
+        if (span.around(row, at - m, 24)) {
+          const uint2* p = reinterpret_cast<const uint2*>(at - m);
+          a = __ldg(p);
+          b = __ldg(p + 1);
+          if (m != 0) c = __ldg(p + 2);
         } else {
-          w[i] = __float_as_uint(v[i]);
+          a = careful<T>(at - m, span.lo, span.hi);
+          b = careful<T>(at - m + 8, span.lo, span.hi);
+          c = careful<T>(at - m + 16, span.lo, span.hi);
         }
       }
     }
+    __device__ __forceinline__ uint4 get() const {
+      if constexpr (WHOLE) {
+        return make_uint4(a.x, a.y, b.x, b.y);
+      } else {
+        uint32_t w[6] = {a.x, a.y, b.x, b.y, c.x, c.y};
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      if (index(h, u) >= H) continue;
-      T* p = row + index(h, u);
-      if constexpr (UNIT == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-      else if constexpr (UNIT == 4) *reinterpret_cast<uint32_t*>(p) = w[u];
-      else *p = static_cast<T>(v[u]);
+        for (int i = 0; i < 5; ++i) w[i] = m & 4 ? w[i + 1] : w[i];
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], m * 8);  // by 0 or 16, modulo 32
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+      }
     }
+
+    // The same of an aligned address.
+    __device__ __forceinline__ void fetch_aligned(const T* first, const Span& span, int row) {
+      if (WHOLE || span.around(row, reinterpret_cast<uintptr_t>(first), 16)) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(first));
+        a = make_uint2(v.x, v.y);
+        b = make_uint2(v.z, v.w);
+      } else {
+        a = careful<T>(reinterpret_cast<uintptr_t>(first), span.lo, span.hi);
+        b = careful<T>(reinterpret_cast<uintptr_t>(first) + 8, span.lo, span.hi);
+      }
+    }
+    __device__ __forceinline__ uint4 get_aligned() const { return make_uint4(a.x, a.y, b.x, b.y); }
+
+  };
+
+  __device__ __forceinline__ static bool inside(int h, int H) { return WHOLE || (h >= 0 && h + kPer<T> <= H); }
+  __device__ __forceinline__ static void store(T* row, int h, int H, const uint4& v) {
+    if (inside(h, H)) {
+      *reinterpret_cast<uint4*>(row + h) = v;
+      return;
+    }
+    // The first or last bytes of the piece, n of them: at most one store of each size.
+    char* p = reinterpret_cast<char*>(row + h);
+    const int size = static_cast<int>(sizeof(T)), n = (h < 0 ? h + kPer<T> : H - h) * size;
+    if (h < 0 && h + kPer<T> <= H) {
+      if (n & 8) *reinterpret_cast<uint2*>(p + 8) = make_uint2(v.z, v.w);
+      if (n & 4) *reinterpret_cast<uint32_t*>(p + (n & 8 ? 4 : 12)) = n & 8 ? v.y : v.w;
+      if constexpr (sizeof(T) == 2)
+        if (n & 2)
+          *reinterpret_cast<uint16_t*>(p + 16 - n) =
+              static_cast<uint16_t>((n & 8 ? (n & 4 ? v.x : v.y) : (n & 4 ? v.z : v.w)) >> 16);
+    } else if (h >= 0) {
+      if (n & 8) *reinterpret_cast<uint2*>(p) = make_uint2(v.x, v.y);
+      if (n & 4) *reinterpret_cast<uint32_t*>(p + (n & 8)) = n & 8 ? v.z : v.x;
+      if constexpr (sizeof(T) == 2)
+        if (n & 2)
+          *reinterpret_cast<uint16_t*>(p + n - 2) = static_cast<uint16_t>(n & 8 ? (n & 4 ? v.w : v.z) : (n & 4 ? v.y : v.x));
+    } else {  // a row that ends in the piece it begins in
+#pragma unroll 1
+      for (int i = -h; i < H - h; ++i) {
+        const uint32_t w = i * size < 8 ? (i * size < 4 ? v.x : v.y) : (i * size < 12 ? v.z : v.w);
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint16_t*>(p + 2 * i) = static_cast<uint16_t>(w >> (16 * (i & 1)));
+        else *reinterpret_cast<uint32_t*>(p + 4 * i) = w;
+      }
+    }
+  }
+  // sum + <d, v> over the columns that exist.
+  __device__ __forceinline__ static float dot(int h, int H, const float (&d)[kPer<T>], const float (&v)[kPer<T>], float sum) {
+    if (inside(h, H)) {
+#pragma unroll
+      for (int i = 0; i < kPer<T>; ++i) sum = fmaf(d[i], v[i], sum);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer<T>; ++i)
+        if (static_cast<unsigned>(h + i) < static_cast<unsigned>(H)) sum = fmaf(d[i], v[i], sum);
+    }
+    return sum;
   }
 };
 
@@ -285,10 +388,11 @@ struct RowArgs {
   int T, K, H, E;
   const int32_t* row_of_pair;
   const int32_t* offsets;
+  int pairs;
   // Row of the token's k-th pair, -1 if it has none.
   __device__ __forceinline__ int64_t row(int64_t t, int k) const {
     const int r = row_of_pair[t * K + k];
-    return r < static_cast<int64_t>(T) * K ? r : -1;
+    return r < pairs ? r : -1;
   }
 };
 
@@ -299,79 +403,106 @@ __device__ __forceinline__ int64_t own_token() {
   return SHORT ? static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y : blockIdx.x;
 }
 
+// A thread's pieces of its token's rows.
+__device__ __forceinline__ int first_piece() { return static_cast<int>(blockIdx.y * blockDim.x + threadIdx.x); }
+__device__ __forceinline__ int piece_stride() { return static_cast<int>(gridDim.y * blockDim.x); }
+
 // The K rows that a token's threads clear if they lie behind the last expert's: rows t * K to t * K + K - 1.
-template <typename T, int UNIT>
+template <typename T, bool WHOLE>
 __device__ __forceinline__ void clear_rows_behind(const RowArgs& a, int64_t t, T* rows) {
-  using P = Piece<T, UNIT>;
+  using C = Cut<T, WHOLE>;
   const int64_t r0 = t * a.K;
-  const float zero[P::kCount] = {};
-  for (int64_t r = max(r0, static_cast<int64_t>(a.offsets[a.E])); r < r0 + a.K; ++r)
-    for (int h = blockIdx.y * P::chunk(); h < a.H; h += gridDim.y * P::chunk()) P::store(rows + r * a.H, h, a.H, zero);
+  for (int64_t r = max(r0, static_cast<int64_t>(a.offsets[a.E])); r < r0 + a.K; ++r) {
+    T* row = rows + r * a.H;
+    for (int p = first_piece(); p < C::pieces(a.H); p += piece_stride()) {
+      const int h = C::column(row, p);
+      if (h < a.H) C::store(row, h, a.H, make_uint4(0, 0, 0, 0));
+    }
+  }
 }
 
-// rows[row_of_pair[t, k]] = hidden[t].  32768 tokens x 4096 bf16, top-8: 2.4 GB in 396 us, the copy rate.
-template <typename T, int UNIT, bool SHORT>
-__global__ void __launch_bounds__(128) sort_rows_kernel(RowArgs a, const T* hidden, int64_t pitch, T* rows) {
-  using P = Piece<T, UNIT>;
+// One piece of a token's row at hidden, into the rows of K pairs; `row_of(k)` is -1 for none.
+template <typename T, bool WHOLE, typename RowOf>
+__device__ __forceinline__ void spread_piece(const RowArgs& a, const T* hidden, const Span& span, int t, int p, T* rows,
+                                             const RowOf& row_of) {
+  using C = Cut<T, WHOLE>;
+  if constexpr (WHOLE) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(hidden + p * kPer<T>));
+    for (int k = 0; k < a.K; ++k) {
+      const int64_t r = row_of(k);
+      if (r >= 0) *reinterpret_cast<uint4*>(rows + r * a.H + p * kPer<T>) = v;
+    }
+  } else {
+    // each lies differently: read, from L1 after the first, as each needs it
+    for (int k = 0; k < a.K; ++k) {
+      const int64_t r = row_of(k);
+      if (r < 0) continue;
+      T* row = rows + r * a.H;
+      const int h = C::column(row, p);
+      if (h >= a.H) continue;
+      typename C::Read piece;
+      piece.fetch(hidden + h, span, t);
+      C::store(row, h, a.H, piece.get());
+    }
+  }
+}
+
+// rows[row_of_pair[t, k]] = hidden[t].  32768 tokens x 4096 bf16, top-8: 2.4 GB in 402 us, 0.92 of the copy rate.
+template <typename T, bool WHOLE, bool SHORT>
+__global__ void __launch_bounds__(128) sort_rows_kernel(RowArgs a, const T* hidden, int64_t pitch, Span span, T* rows) {
   grid_enter(a.row_of_pair, a.offsets, hidden);
   const int64_t t = own_token<SHORT>();
   if (SHORT && t >= a.T) return;
-  for (int h = blockIdx.y * P::chunk(); h < a.H; h += gridDim.y * P::chunk()) {
-    P piece;
-    float v[P::kCount];
-    piece.fetch(hidden + t * pitch, h, a.H);
-    piece.values(v);
-    for (int k = 0; k < a.K; ++k) {
-      const int64_t r = a.row(t, k);
-      if (r >= 0) P::store(rows + r * a.H, h, a.H, v);
-    }
-  }
-  clear_rows_behind<T, UNIT>(a, t, rows);
+  for (int p = first_piece(); p < Cut<T, WHOLE>::pieces(a.H); p += piece_stride())
+    spread_piece<T, WHOLE>(a, hidden + t * pitch, span, static_cast<int>(t), p, rows, [&](int k) { return a.row(t, k); });
+  clear_rows_behind<T, WHOLE>(a, t, rows);
 }
 
 // Order and rows in one launch for a few tokens: every CTA works the order out for itself and moves one token's rows.
-template <typename T, int UNIT>
-__global__ void __launch_bounds__(kSortThreads) sort_few_kernel(SortArgs s, RowArgs a, const T* hidden, int64_t pitch,
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(kSortThreads) sort_few_kernel(SortArgs s, RowArgs a, const T* hidden, int64_t pitch, Span span,
                                                                 int32_t* offsets, int32_t* row_of_pair, T* rows) {
-  using P = Piece<T, UNIT>;
+  using C = Cut<T, WHOLE>;
   extern __shared__ int hist[];
   __shared__ int s_row[kChunk];
   grid_enter(s.index, hidden);
   const bool first = blockIdx.x == 0;
   const int64_t t = blockIdx.x;
-  P piece;  // on its way while the order is worked out
-  piece.fetch(hidden + t * pitch, 0, a.H);
+  // on its way while the order is worked out
+  if (static_cast<int>(threadIdx.x) * kPer<T> < a.H)
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(hidden + t * pitch + threadIdx.x * kPer<T>));
   const int used = order_chunk(s, 0, 1, nullptr, false, hist, first ? offsets : nullptr, [&](int64_t p, int row) {
     s_row[p] = row;
     if (first) row_of_pair[p] = row;
   });
   __syncthreads();
-  const float zero[P::kCount] = {};
-  for (int h = 0; h < a.H; h += P::chunk()) {
-    float v[P::kCount];
-    if (h > 0) piece.fetch(hidden + t * pitch, h, a.H);
-    piece.values(v);
-    for (int k = 0; k < a.K; ++k) {
-      const int r = s_row[t * a.K + k];
-      if (r >= 0) P::store(rows + static_cast<int64_t>(r) * a.H, h, a.H, v);
-      if (t * a.K + k >= used) P::store(rows + (t * a.K + k) * a.H, h, a.H, zero);  // this row lies behind the last expert's
+  for (int p = threadIdx.x; p < C::pieces(a.H); p += kSortThreads)
+    spread_piece<T, WHOLE>(a, hidden + t * pitch, span, static_cast<int>(t), p, rows,
+                           [&](int k) -> int64_t { return s_row[t * a.K + k]; });
+  for (int64_t r = max(t * a.K, static_cast<int64_t>(used)); r < (t + 1) * a.K; ++r) {  // behind the last expert's rows
+    for (int p = threadIdx.x; p < C::pieces(a.H); p += kSortThreads) {
+      const int h = C::column(rows + r * a.H, p);
+      if (h < a.H) C::store(rows + r * a.H, h, a.H, make_uint4(0, 0, 0, 0));
     }
   }
 }
 
 // out[t] = sum over k of (affinities[t, k]) rows[row_of_pair[t, k]], in fp32, k ascending, rounded once.  The same 2.4 GB in
-// 356 us (343 without weights); one row at a time, 400 (386).
-template <typename T, int UNIT, bool SHORT, int ROWS>
-__global__ void __launch_bounds__(128) unsort_rows_kernel(RowArgs a, const T* rows, int64_t pitch, const void* affinities,
-                                                          int aff_dtype, T* out) {
-  using P = Piece<T, UNIT>;
+// 351 us (341 without weights); one row at a time, 400 (386).
+template <typename T, bool WHOLE, bool SHORT, int ROWS>
+__global__ void __launch_bounds__(128, !WHOLE && SHORT ? 8 : 0)  // 80 registers without the bound, 123 us instead of 106 at 130 columns
+unsort_rows_kernel(RowArgs a, const T* rows, int64_t pitch, Span span, const void* affinities, int aff_dtype, T* out) {
+  using C = Cut<T, WHOLE>;
   grid_enter(a.row_of_pair, rows, affinities);
   const int64_t t = own_token<SHORT>();
   if (SHORT && t >= a.T) return;
-  for (int h = blockIdx.y * P::chunk(); h < a.H; h += gridDim.y * P::chunk()) {
-    float sum[P::kCount] = {};
+  T* to = out + t * a.H;
+  for (int p = first_piece(); p < C::pieces(a.H); p += piece_stride()) {
+    const int h = C::column(to, p);
+    if (h >= a.H) break;
+    float sum[kPer<T>] = {};
     for (int k0 = 0; k0 < a.K; k0 += ROWS) {  // ROWS rows on their way before the first is added
-      P piece[ROWS];
+      typename C::Read piece[ROWS];
       float w[ROWS];
       bool live[ROWS];
 #pragma unroll
@@ -379,101 +510,142 @@ __global__ void __launch_bounds__(128) unsort_rows_kernel(RowArgs a, const T* ro
         const int64_t r = k0 + j < a.K ? a.row(t, k0 + j) : -1;
         live[j] = r >= 0;
         if (!live[j]) continue;
-        piece[j].fetch(rows + r * pitch, h, a.H);
+        piece[j].fetch(rows + r * pitch + h, span, static_cast<int>(r));
         w[j] = affinities != nullptr ? load_as_float(affinities, t * a.K + k0 + j, aff_dtype) : 1.0f;
       }
 #pragma unroll
       for (int j = 0; j < ROWS; ++j) {
         if (!live[j]) continue;
-        float v[P::kCount];
-        piece[j].values(v);
+        float v[kPer<T>];
+        unpack<T>(piece[j].get(), v);
 #pragma unroll
-        for (int i = 0; i < P::kCount; ++i) sum[i] = fmaf(w[j], v[i], sum[i]);
+        for (int i = 0; i < kPer<T>; ++i) sum[i] = fmaf(w[j], v[i], sum[i]);
       }
     }
-    P::store(out + t * a.H, h, a.H, sum);
+    C::store(to, h, a.H, pack<T>(sum));
   }
 }
 
+// Lane j's result is the sum of v[j] over the warp (j < N, a power of two): lanes share the values out as they add them up.
+template <int N>
+__device__ __forceinline__ float sum_over_warp(float (&v)[N], int lane) {
+#pragma unroll
+  for (int n = N / 2; n > 0; n >>= 1) {
+    const bool upper = lane & n;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float other = __shfl_xor_sync(0xffffffffu, upper ? v[i] : v[i + n], n);
+      v[i] = (upper ? v[i + n] : v[i]) + other;
+    }
+  }
+#pragma unroll
+  for (int o = N; o < 32; o <<= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  return v[0];
+}
+
 // d rows[r] = a[t, k] d out[t]; d a[t, k] = <d out[t], rows[r]>: one pass over a token's rows for both.  32768 tokens x 4096
-// bf16, top-8: 4.6 GB in 695 us; with a row's load, product and store one after the other 1121.
-template <typename T, int UNIT, bool SHORT, int ROWS>
-__global__ void __launch_bounds__(256) unsort_backward_kernel(RowArgs a, const T* d_out, int64_t d_pitch, const T* rows,
-                                                              int64_t pitch, const void* affinities, int aff_dtype,
-                                                              T* d_rows, void* d_affinities) {
-  using P = Piece<T, UNIT>;
-  __shared__ float s_dot[8][ROWS];
+// bf16, top-8: 4.6 GB in 687 us; with a row's load, product and store one after the other 1121.  ALIKE: a row that is read and the
+// one that is written in its place lie alike in their 16 bytes (or only one of them is there).
+// The cut form lives from occupancy (48 or 64 registers; unbounded at 100, 6000 x 5003, top-8: 334 us, 209 so), the whole one from
+// the rows in flight.
+template <typename T, bool WHOLE, bool ALIKE, bool SHORT, int ROWS>
+__global__ void __launch_bounds__(256, WHOLE || ROWS > 4 ? 0 : (ALIKE && ROWS == 2 ? 5 : 4))
+unsort_backward_kernel(RowArgs a, const T* d_out, int64_t d_pitch, Span d_span, const T* rows, int64_t pitch, Span span,
+                       const void* affinities, int aff_dtype, T* d_rows, void* d_affinities) {
+  using C = Cut<T, WHOLE>;
+  __shared__ float s_dot[2][8][ROWS];
   grid_enter(a.row_of_pair, a.offsets, d_out, rows, affinities);
   const int64_t t = own_token<SHORT>();
   const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;  // of a token
   const int warp0 = SHORT ? threadIdx.y * warps : 0, warp = warp0 + (threadIdx.x >> 5);
-  for (int k0 = 0; k0 < a.K; k0 += ROWS) {
+  int buffer = 0;  // of s_dot: with two, one barrier per ROWS rows
+  for (int k0 = 0; k0 < a.K; k0 += ROWS, buffer ^= 1) {
     const int n = !SHORT || t < a.T ? min(ROWS, a.K - k0) : 0;
-    int64_t r[ROWS];
+    int r[ROWS];
     float w[ROWS], dot[ROWS];
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
-      r[j] = j < n ? a.row(t, k0 + j) : -1;
+      r[j] = j < n ? static_cast<int>(a.row(t, k0 + j)) : -1;
       w[j] = j < n && affinities != nullptr ? load_as_float(affinities, t * a.K + k0 + j, aff_dtype) : 1.0f;
       dot[j] = 0.f;
     }
-    for (int h = 0; h < a.H && n > 0; h += P::chunk()) {
-      P piece[ROWS], own;  // all rows on their way before the first is used
-      own.fetch(d_out + t * d_pitch, h, a.H);
+    // One piece of row j: what `d` of the gradient and `piece` of the row give.
+    const auto use = [&](int j, int h, const float (&d)[kPer<T>], const uint4& piece) {
+      float v[kPer<T>];
       if (d_affinities != nullptr) {
+        unpack<T>(piece, v);
+        dot[j] = C::dot(h, a.H, d, v, dot[j]);
+      }
+      if (d_rows != nullptr) {
+#pragma unroll
+        for (int i = 0; i < kPer<T>; ++i) v[i] = w[j] * d[i];
+        C::store(d_rows + static_cast<int64_t>(r[j]) * a.H, h, a.H, pack<T>(v));
+      }
+    };
+    for (int p = threadIdx.x; p < C::pieces(a.H) && n > 0; p += blockDim.x) {
+      typename C::Read piece[ROWS];  // all rows on their way before the first is used
+      if constexpr (WHOLE) {
+        const int h = p * kPer<T>;
+        typename C::Read own;
+        own.fetch_aligned(d_out + t * d_pitch + h, d_span, 0);
+        if (d_affinities != nullptr) {
+#pragma unroll
+          for (int j = 0; j < ROWS; ++j)
+            if (r[j] >= 0) piece[j].fetch_aligned(rows + static_cast<int64_t>(r[j]) * pitch + h, span, 0);
+        }
+        float d[kPer<T>];
+        unpack<T>(own.get_aligned(), d);
 #pragma unroll
         for (int j = 0; j < ROWS; ++j)
-          if (r[j] >= 0) piece[j].fetch(rows + r[j] * pitch, h, a.H);
-      }
-      float d[P::kCount];
-      own.values(d);
+          if (r[j] >= 0) use(j, h, d, piece[j].get_aligned());
+      } else {
+        // cut as the row that is written; the gradient's pieces then differ from row to row and come from L1 after the first
+        typename C::Read own[2];
+        int h[ROWS];
 #pragma unroll
-      for (int j = 0; j < ROWS; ++j) {
-        if (r[j] < 0) continue;
-        float v[P::kCount];
-        if (d_affinities != nullptr) {
-          piece[j].values(v);
-#pragma unroll
-          for (int i = 0; i < P::kCount; ++i) dot[j] = fmaf(d[i], v[i], dot[j]);
+        for (int j = 0; j < ROWS; ++j) {
+          h[j] = a.H;
+          if (r[j] < 0) continue;
+          const T* row = rows + static_cast<int64_t>(r[j]) * pitch;
+          h[j] = C::column(d_rows != nullptr ? d_rows + static_cast<int64_t>(r[j]) * a.H : row, p);
+          if (h[j] >= a.H || d_affinities == nullptr) continue;
+          if constexpr (ALIKE) piece[j].fetch_aligned(row + h[j], span, r[j]);
+          else piece[j].fetch(row + h[j], span, r[j]);
         }
-        if (d_rows != nullptr) {
+        if (h[0] < a.H) own[0].fetch(d_out + t * d_pitch + h[0], d_span, static_cast<int>(t));
 #pragma unroll
-          for (int i = 0; i < P::kCount; ++i) v[i] = w[j] * d[i];
-          P::store(d_rows + r[j] * a.H, h, a.H, v);
+        for (int j = 0; j < ROWS; ++j) {
+          if (j + 1 < ROWS && h[j + 1 < ROWS ? j + 1 : 0] < a.H)
+            own[(j + 1) & 1].fetch(d_out + t * d_pitch + h[j + 1 < ROWS ? j + 1 : 0], d_span, static_cast<int>(t));
+          if (h[j] >= a.H) continue;
+          float d[kPer<T>];
+          unpack<T>(own[j & 1].get(), d);
+          use(j, h[j], d, ALIKE ? piece[j].get_aligned() : piece[j].get());
         }
       }
     }
     if (d_affinities != nullptr) {
-#pragma unroll
-      for (int j = 0; j < ROWS; ++j) {
-        float s = dot[j];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) s_dot[warp][j] = s;
-      }
+      const float s = sum_over_warp<ROWS>(dot, lane);
+      if (lane < ROWS) s_dot[buffer][warp][lane] = s;
       __syncthreads();
       if (threadIdx.x < static_cast<unsigned>(n)) {
         float s = 0.f;
-        for (int i = 0; i < warps; ++i) s += s_dot[warp0 + i][threadIdx.x];
+        for (int i = 0; i < warps; ++i) s += s_dot[buffer][warp0 + i][threadIdx.x];
         store_from_float(d_affinities, t * a.K + k0 + threadIdx.x, aff_dtype, s);
       }
-      __syncthreads();
     }
   }
-  if (d_rows != nullptr && (!SHORT || t < a.T)) clear_rows_behind<T, UNIT>(a, t, d_rows);
+  if (d_rows != nullptr && (!SHORT || t < a.T)) clear_rows_behind<T, WHOLE>(a, t, d_rows);
 }
 
-// Bytes that the rows of all given matrices can be moved by: 16, 4, or an element's.
 struct Rows {
   const void* p;
   int64_t pitch;
 };
-int common_unit(int dtype, int H, std::initializer_list<Rows> matrices) {
-  const int size = dtype == B200MOE_F32 ? 4 : 2;
-  uint64_t bits = static_cast<uint64_t>(H) * size;
-  for (const Rows& m : matrices)
-    if (m.p != nullptr) bits |= reinterpret_cast<uintptr_t>(m.p) | static_cast<uint64_t>(m.pitch * size);
-  return bits % 16 == 0 ? 16 : (bits % 4 == 0 ? 4 : size);
+Span span_of(int dtype, const void* p, int64_t rows, int64_t pitch, int H) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(p), size = dtype == B200MOE_F32 ? 4 : 2;
+  const bool apart = pitch >= H && H * size >= 32 && rows > 2;
+  return {lo, lo + static_cast<uintptr_t>((rows - 1) * pitch + H) * size, 1, apart ? static_cast<unsigned>(rows - 2) : 0u};
 }
 
 // With enough tokens to give every SM several CTAs, a CTA of `threads` has as many tokens as their rows leave room for (30000
@@ -510,14 +682,21 @@ int check_sort(const void* expert_index, int index_bytes, int T, int K, int E, c
   return B200MOE_OK;
 }
 
-// Calls fn with a value of the element type and the unit its rows move by, both known to the compiler.
+// Calls fn with a value of the element type and whether all rows of the matrices are whole aligned 16 bytes, both known to the
+// compiler.
 template <typename F>
-int with_rows(int dtype, int unit, const F& fn) {
-  using std::integral_constant;
-  if (dtype == B200MOE_F32)
-    return unit == 16 ? fn(float{}, integral_constant<int, 16>{}) : fn(float{}, integral_constant<int, 4>{});
-  if (unit == 16) return fn(__nv_bfloat16{}, integral_constant<int, 16>{});
-  return unit == 4 ? fn(__nv_bfloat16{}, integral_constant<int, 4>{}) : fn(__nv_bfloat16{}, integral_constant<int, 2>{});
+int with_rows(const char* name, int dtype, int H, std::initializer_list<Rows> matrices, const F& fn) {
+  const int size = dtype == B200MOE_F32 ? 4 : 2;
+  uint64_t at = 0, apart = static_cast<uint64_t>(H) * size;
+  for (const Rows& m : matrices) {
+    if (m.p == nullptr) continue;
+    at |= reinterpret_cast<uintptr_t>(m.p);
+    apart |= static_cast<uint64_t>(m.pitch * size);
+  }
+  B200MOE_REQUIRE(at % size == 0, B200MOE_ERR_INVALID, "%s: rows must start on an element's boundary", name);
+  const bool whole = (at | apart) % 16 == 0;
+  if (dtype == B200MOE_F32) return whole ? fn(float{}, std::true_type{}) : fn(float{}, std::false_type{});
+  return whole ? fn(__nv_bfloat16{}, std::true_type{}) : fn(__nv_bfloat16{}, std::false_type{});
 }
 
 }  // namespace
@@ -565,14 +744,14 @@ extern "C" int b200moe_sort_rows(const void* hidden, int dtype, int64_t pitch, i
   int rc = check_rows("sort_rows", dtype, T, K, H, pitch);
   if (rc != B200MOE_OK) return rc;
   B200MOE_REQUIRE(E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID, "sort_rows: between 1 and %d experts, got %d", kMaxExperts, E);
-  const RowArgs a{T, K, H, E, row_of_pair, expert_offsets};
-  return with_rows(dtype, common_unit(dtype, H, {{hidden, pitch}, {rows, H}}), [&](auto element, auto width) -> int {
+  const RowArgs a{T, K, H, E, row_of_pair, expert_offsets, T * K};
+  return with_rows("sort_rows", dtype, H, {{hidden, pitch}, {rows, H}}, [&](auto element, auto whole) -> int {
     using T_ = decltype(element);
-    constexpr int U = decltype(width)::value;
-    const Layout l = row_layout(T, H, Piece<T_, U>::kCount, 128, true);
-    const auto kernel = l.block.y > 1 ? sort_rows_kernel<T_, U, true> : sort_rows_kernel<T_, U, false>;
+    constexpr bool W = decltype(whole)::value;
+    const Layout l = row_layout(T, H, kPer<T_>, 128, true);
+    const auto kernel = l.block.y > 1 ? sort_rows_kernel<T_, W, true> : sort_rows_kernel<T_, W, false>;
     B200MOE_CUDA_OK(launch_overlapped(kernel, l.grid, l.block, 0, static_cast<cudaStream_t>(stream), a,
-                                      static_cast<const T_*>(hidden), pitch, static_cast<T_*>(rows)));
+                                      static_cast<const T_*>(hidden), pitch, span_of(dtype, hidden, T, pitch, H), static_cast<T_*>(rows)));
     B200MOE_LAUNCH_OK("sort_rows_kernel");
     return B200MOE_OK;
   });
@@ -590,13 +769,14 @@ extern "C" int b200moe_sort_tokens(const void* hidden, int dtype, int64_t pitch,
   // instead of 4.8 + 3.8, and 16.6 instead of 19.3 of host time)
   if (static_cast<int64_t>(T) * K <= kChunk && T <= 128) {
     const SortArgs s{expert_index, index_bytes == 8, static_cast<int64_t>(T) * K, E};
-    const RowArgs a{T, K, H, E, nullptr, nullptr};
-    return with_rows(dtype, common_unit(dtype, H, {{hidden, pitch}, {rows, H}}), [&](auto element, auto width) -> int {
+    const RowArgs a{T, K, H, E, nullptr, nullptr, T * K};
+    return with_rows("sort_tokens", dtype, H, {{hidden, pitch}, {rows, H}}, [&](auto element, auto whole) -> int {
       using T_ = decltype(element);
-      constexpr int U = decltype(width)::value;
-      B200MOE_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(sort_few_kernel<T_, U>), kMostHist));
-      B200MOE_CUDA_OK(launch_overlapped(sort_few_kernel<T_, U>, dim3(T), kSortThreads, (kSortWarps + 1) * E * sizeof(int),
+      constexpr bool W = decltype(whole)::value;
+      B200MOE_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(sort_few_kernel<T_, W>), kMostHist));
+      B200MOE_CUDA_OK(launch_overlapped(sort_few_kernel<T_, W>, dim3(T), kSortThreads, (kSortWarps + 1) * E * sizeof(int),
                                         static_cast<cudaStream_t>(stream), s, a, static_cast<const T_*>(hidden), pitch,
+                                        span_of(dtype, hidden, T, pitch, H),
                                         expert_offsets, row_of_pair, static_cast<T_*>(rows)));
       B200MOE_LAUNCH_OK("sort_few_kernel");
       return B200MOE_OK;
@@ -614,15 +794,17 @@ extern "C" int b200moe_unsort_rows(const void* rows, int dtype, int64_t pitch, i
   if (rc != B200MOE_OK) return rc;
   B200MOE_REQUIRE(affinities == nullptr || aff_dtype == B200MOE_F32 || aff_dtype == B200MOE_BF16, B200MOE_ERR_INVALID,
                   "unsort_rows: affinities must be fp32 or bf16");
-  const RowArgs a{T, K, H, 0, row_of_pair, nullptr};
-  return with_rows(dtype, common_unit(dtype, H, {{rows, pitch}, {out, H}}), [&](auto element, auto width) -> int {
+  const RowArgs a{T, K, H, 0, row_of_pair, nullptr, T * K};
+  return with_rows("unsort_rows", dtype, H, {{rows, pitch}, {out, H}}, [&](auto element, auto whole) -> int {
     using T_ = decltype(element);
-    constexpr int U = decltype(width)::value;
-    const Layout l = row_layout(T, H, Piece<T_, U>::kCount, 128, true);
-    const auto kernel = l.block.y > 1 ? (K > 4 ? unsort_rows_kernel<T_, U, true, 8> : unsort_rows_kernel<T_, U, true, 4>)
-                                      : (K > 4 ? unsort_rows_kernel<T_, U, false, 8> : unsort_rows_kernel<T_, U, false, 4>);
+    constexpr bool W = decltype(whole)::value;
+    const Layout l = row_layout(T, H, kPer<T_>, 128, true);
+    const auto kernel = l.block.y > 1 ? (K > 4 ? unsort_rows_kernel<T_, W, true, W ? 8 : 4> : unsort_rows_kernel<T_, W, true, 4>)
+                                      : (K > 4 ? unsort_rows_kernel<T_, W, false, W ? 8 : 4> : unsort_rows_kernel<T_, W, false, 4>);
     B200MOE_CUDA_OK(launch_overlapped(kernel, l.grid, l.block, 0, static_cast<cudaStream_t>(stream), a,
-                                      static_cast<const T_*>(rows), pitch, affinities, aff_dtype, static_cast<T_*>(out)));
+                                      static_cast<const T_*>(rows), pitch,
+                                      span_of(dtype, rows, static_cast<int64_t>(T) * K, pitch, H), affinities,
+                                      aff_dtype, static_cast<T_*>(out)));
     B200MOE_LAUNCH_OK("unsort_rows_kernel");
     return B200MOE_OK;
   });
@@ -643,20 +825,31 @@ extern "C" int b200moe_unsort_rows_backward(const void* d_out, int64_t d_pitch, 
                   "unsort_rows_backward: affinities must be fp32 or bf16");
   B200MOE_REQUIRE(E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID, "unsort_rows_backward: between 1 and %d experts, got %d",
                   kMaxExperts, E);
-  const RowArgs a{T, K, H, E, row_of_pair, expert_offsets};
-  return with_rows(dtype, common_unit(dtype, H, {{d_out, d_pitch}, {rows, pitch}, {d_rows, H}}), [&](auto element, auto width) -> int {
+  const RowArgs a{T, K, H, E, row_of_pair, expert_offsets, T * K};
+  return with_rows("unsort_rows_backward", dtype, H, {{d_out, d_pitch}, {rows, pitch}, {d_rows, H}},
+                   [&](auto element, auto whole) -> int {
     using T_ = decltype(element);
-    constexpr int U = decltype(width)::value;
-    const int threads = T >= 8 * sm_count() && H <= 128 * 4 * Piece<T_, U>::kCount ? 128 : 256;
-    const Layout l = row_layout(T, H, Piece<T_, U>::kCount, threads, false);
-    const auto pick = [&](auto few) {
-      constexpr bool S = decltype(few)::value;
-      return K > 4 ? unsort_backward_kernel<T_, U, S, 8>
-                   : (K > 2 ? unsort_backward_kernel<T_, U, S, 4> : unsort_backward_kernel<T_, U, S, 2>);
+    constexpr bool W = decltype(whole)::value;
+    const int threads = T >= 8 * sm_count() && H <= 128 * 8 * kPer<T_> ? 128 : 256;
+    const Layout l = row_layout(T, H, kPer<T_>, threads, false);
+    const bool few_tokens = T <= 2 * sm_count();  // all of them at once in the form of eight rows
+    const auto pick = [&](auto brief, auto alike) {
+      constexpr bool S = decltype(brief)::value, A = decltype(alike)::value;
+      if (!A || K <= 2 || (!W && S)) return unsort_backward_kernel<T_, W, A, S, 2>;
+      if constexpr (A && (W || !S))
+        return K > 4 && (W || few_tokens) ? unsort_backward_kernel<T_, W, A, S, 8> : unsort_backward_kernel<T_, W, A, S, 4>;
+      return unsort_backward_kernel<T_, W, A, S, 2>;
     };
-    const auto kernel = l.block.y > 1 ? pick(std::true_type{}) : pick(std::false_type{});
+    const auto with_length = [&](auto alike) {
+      return l.block.y > 1 ? pick(std::true_type{}, alike) : pick(std::false_type{}, alike);
+    };
+    const bool lie_alike = d_rows == nullptr || d_affinities == nullptr ||
+                           (((reinterpret_cast<uintptr_t>(rows) ^ reinterpret_cast<uintptr_t>(d_rows)) |
+                             static_cast<uintptr_t>((pitch - H) * static_cast<int64_t>(sizeof(T_)))) & 15) == 0;
+    const auto kernel = W || lie_alike ? with_length(std::true_type{}) : with_length(std::bool_constant<W>{});
     B200MOE_CUDA_OK(launch_overlapped(kernel, l.grid, l.block, 0, static_cast<cudaStream_t>(stream), a,
-                                      static_cast<const T_*>(d_out), d_pitch, static_cast<const T_*>(rows), pitch, affinities,
+                                      static_cast<const T_*>(d_out), d_pitch, span_of(dtype, d_out, T, d_pitch, H),
+                                      static_cast<const T_*>(rows), pitch, span_of(dtype, rows, static_cast<int64_t>(T) * K, pitch, H), affinities,
                                       aff_dtype, static_cast<T_*>(d_rows), d_affinities));
     B200MOE_LAUNCH_OK("unsort_backward_kernel");
     return B200MOE_OK;

@@ -186,6 +186,74 @@ def test_rows_with_other_strides():
     assert all(torch.equal(g, w) for g, w in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,K,E", [(1, 1, 1), (2, 2, 3), (9, 3, 4), (200, 5, 8), (1300, 2, 8)])
+@pytest.mark.parametrize("H", [1, 2, 3, 5, 8, 9, 15, 17, 31, 130, 257, 1001])
+def test_rows_at_any_address(T, K, E, H, dtype):
+    """Matrices anywhere between elements that are not theirs: NaN around every row that is read reaches no result, and what
+    surrounds the rows that are written stays as it was."""
+    from nki_library_b200 import _lib
+    from nki_library_b200.core.moe.moe_train.launch import launch
+    import nki_library_b200 as m
+    gen = _gen(T + H)
+    idx = _ids(T, K, E, H, 0.1)
+    plan = m.moe_sort_plan(idx, E)
+    row, used = plan.row_of_pair, int(plan.expert_offsets[-1])
+    device, code = row.device, _lib.BF16 if dtype == torch.bfloat16 else _lib.F32
+    MARK = -77.0
+
+    def surrounded(rows, offset, gap, fill):
+        flat = torch.full((offset + rows * (H + gap) + 40,), fill, dtype=dtype, device=device)
+        return flat, flat[offset:].as_strided((rows, H), (H + gap, 1))
+
+    def untouched(flat, view):
+        view.fill_(MARK)
+        return bool((flat == MARK).all())
+
+    a = torch.rand((T, K), device=device, generator=gen)
+    live = (row >= 0).flatten()
+    token = (torch.arange(T * K, device=device) // K)[live]
+    to = row.flatten()[live].long()
+    for offset, gap in ((0, 0), (1, 0), (3, 2), (6, 0), (7, 9), (8, 16)):
+        _, hidden = surrounded(T, offset, gap, float("nan"))
+        _, y = surrounded(T * K, offset + 1, gap, float("nan"))
+        hidden.copy_(torch.randn((T, H), device=device, generator=gen))
+        y.copy_(torch.randn((T * K, H), device=device, generator=gen))
+        y[used:] = float("nan")  # rows of no expert
+        flat, rows = surrounded(T * K, 8 - offset, 0, MARK)
+        launch(device, "b200moe_sort_rows", hidden.data_ptr(), code, H + gap, T, K, H, E, row.data_ptr(),
+               plan.expert_offsets.data_ptr(), rows.data_ptr())
+        want = torch.zeros((T * K, H), dtype=dtype, device=device)
+        want[to] = hidden[token]
+        assert torch.equal(rows, want) and untouched(flat, rows)
+        if T <= 128:
+            off, row2 = torch.empty_like(plan.expert_offsets), torch.empty_like(row)
+            launch(device, "b200moe_sort_tokens", hidden.data_ptr(), code, H + gap, idx.data_ptr(), 4, T, K, H, E, off.data_ptr(),
+                   row2.data_ptr(), rows.data_ptr(), None, 0)
+            assert torch.equal(rows, want) and torch.equal(row2, row) and untouched(flat, rows)
+        flat, out = surrounded(T, offset, 0, MARK)
+        launch(device, "b200moe_unsort_rows", y.data_ptr(), code, H + gap, T, K, H, row.data_ptr(), a.data_ptr(), _lib.F32,
+               out.data_ptr())
+        terms = y.double()[to] * a.double().flatten()[live][:, None]
+        zero = torch.zeros((T, H), dtype=torch.float64, device=device)
+        _close(out, zero.index_add(0, token, terms), zero.index_add(0, token, terms.abs()), K)
+        assert untouched(flat, out)
+        for lie in (offset + 1, offset):  # like the rows that are read, and not
+            flat, d_rows = surrounded(T * K, lie, 0, MARK)
+            d_a = torch.empty_like(a)
+            launch(device, "b200moe_unsort_rows_backward", hidden.data_ptr(), H + gap, y.data_ptr(), H + gap, code, T, K, H, E,
+                   row.data_ptr(), plan.expert_offsets.data_ptr(), a.data_ptr(), _lib.F32, d_rows.data_ptr(), d_a.data_ptr())
+            want = torch.zeros((T * K, H), dtype=torch.float64, device=device)
+            want[to] = hidden.double()[token] * a.double().flatten()[live][:, None]
+            _close(d_rows, want, want.abs(), 1)
+            assert untouched(flat, d_rows)
+            products = hidden.double()[token] * y.double()[to]
+            want = torch.zeros(T * K, dtype=torch.float64, device=device)
+            size = want.clone()
+            want[live], size[live] = products.sum(1), products.abs().sum(1)
+            _close(d_a.flatten(), want, size, H)
+
+
 def test_sums_and_their_gradients_agree_with_differences():
     """Both directions are linear in their rows and affinities: fp32 differences against the gradients."""
     import nki_library_b200 as m

@@ -61,13 +61,17 @@ def test_entry_points_refuse(name, args, code, message):
 @pytest.mark.parametrize("name,args,message", [
     ("b200moe_sort_tokens", (P, 1, 8, P, 4, 4, 2, (1 << 30) + 8, 8, P, P, P, None, 0, None), "2^30 columns"),
     ("b200moe_unsort_rows", (P, 1, 8, 4, 2, (1 << 30) + 8, P, None, 0, P, None), "2^30 columns"),
+    ("b200moe_sort_rows", (P + 1, 1, 8, 4, 2, 8, 8, P, P, P, None), "element's boundary"),
+    ("b200moe_sort_tokens", (P, 0, 8, P, 4, 4, 2, 8, 8, P, P, P + 2, None, 0, None), "element's boundary"),
+    ("b200moe_unsort_rows", (P, 1, 8, 4, 2, 8, P, None, 0, P + 1, None), "element's boundary"),
+    ("b200moe_unsort_rows_backward", (P, 8, P, 8, 0, 4, 2, 8, 8, P, P, P, 0, P + 6, P, None), "element's boundary"),
     ("b200moe_expert_product", (P, 64, P, 64, 4096, 0, P, (1 << 30) + 1, 2, 64, 64, P, None, 0, P, None), "2^30"),
     ("b200moe_expert_product", (P, 1 << 28, P, 64, 1 << 35, 0, P, 8, 2, 1 << 28, 64, P, None, 0, P, None), "2^27"),
     ("b200moe_expert_product", (P, 64, P, 1 << 28, 1 << 35, 0, P, 8, 2, 64, 1 << 28, P, None, 0, P, None), "2^27"),
     ("b200moe_expert_weight_grad", (P, 64, P, 64, P, (1 << 30) + 1, 2, 64, 64, P, None, 0, P, None), "2^30"),
     ("b200moe_expert_weight_grad", (P, 1 << 28, P, 64, P, 8, 2, 1 << 28, 64, P, None, 0, P, None), "2^27"),
 ])
-def test_sizes_whose_indices_would_overflow_are_refused(name, args, message):
+def test_sizes_and_addresses_without_an_index_are_refused(name, args, message):
     rc, text = _refused(name, *args)
     assert rc == -1 and message in text, (rc, text)
 
