@@ -1,13 +1,15 @@
-"""Build the CUDA shared library in-tree with nvcc for sm_100a.
+"""Build the CUDA shared library in-tree with nvcc for sm_100a, and the torch side of the training operators with g++.
 
 ``python -m nki_library_b200.build`` (or ``build_library()``) compiles every
-``csrc/*.cu`` into ``nki_library_b200/libb200moe.so``.  nvcc cross-compiles, so
-this works on a machine without a GPU.
+``csrc/*.cu`` into ``nki_library_b200/libb200moe.so``, and ``csrc/autograd.cpp``
+against it into ``nki_library_b200/_autograd.so``.  nvcc cross-compiles, so this
+works on a machine without a GPU.
 """
 
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
@@ -15,6 +17,7 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libb200moe.so")
+AUTOGRAD = os.path.join(PKG, "_autograd.so")
 BUILD = os.path.join(PKG, "build")
 
 NVCC_FLAGS = [
@@ -35,6 +38,27 @@ def _stale(target: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _autograd_compile(source: str, target: str) -> list:
+    import sysconfig
+
+    import torch
+
+    include = os.path.join(os.path.dirname(torch.__file__), "include")
+    dirs = [include, os.path.join(include, "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
+            os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")]
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-DTORCH_EXTENSION_NAME=_autograd",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"] +
+            [a for d in dirs for a in ("-isystem", d)] + ["-c", source, "-o", target])
+
+
+def _autograd_link(target: str) -> list:
+    import torch
+
+    return ["g++", "-shared", "-o", AUTOGRAD, target, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"),
+            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10", "-L" + PKG, "-l:" + os.path.basename(LIB),
+            "-Wl,-rpath,$ORIGIN"]
+
+
 def build_library(force: bool = False, verbose: bool = False) -> str:
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
     hdrs = sorted(glob.glob(os.path.join(CSRC, "*.cuh"))) + [os.path.join(os.path.dirname(PKG), "include", "b200moe.h")]
@@ -47,6 +71,11 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
         if force or _stale(o, [s] + hdrs):
             cmd = [_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", s, "-o", o]
             procs.append((s, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    source, autograd = os.path.join(CSRC, "autograd.cpp"), os.path.join(BUILD, "autograd.o")
+    torch = importlib.util.find_spec("torch") is not None  # a C program needs neither it nor this part
+    if torch and (force or _stale(autograd, [source, hdrs[-1]])):
+        procs.append((source, subprocess.Popen(_autograd_compile(source, autograd), stdout=subprocess.PIPE,
+                                               stderr=subprocess.STDOUT, text=True)))
     failed = False
     for s, p in procs:
         out, _ = p.communicate()
@@ -54,9 +83,11 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
             sys.stderr.write(out)
         failed |= p.returncode != 0
     if failed:
-        raise RuntimeError("nvcc failed")
+        raise RuntimeError("compilation failed")
     if force or procs or _stale(LIB, objs):
         subprocess.check_call([_nvcc(), "-shared", "-o", LIB] + objs + ["-lcudart"])
+    if torch and (force or _stale(AUTOGRAD, [autograd])):
+        subprocess.check_call(_autograd_link(autograd))
     return LIB
 
 

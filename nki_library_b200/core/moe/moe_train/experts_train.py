@@ -6,32 +6,9 @@ import torch
 
 from .... import _lib
 from ...utils.common_types import ActFnType
-from .expert_linear import MOST_COLUMNS, check_rows_and_weight, product, weight_grad
-from .launch import needs_grad, once, same_device, tile_rows
-from .moe_glu import glu_backward, glu_forward
+from .expert_linear import MOST_COLUMNS, check_rows_and_weight
+from .launch import native, same_device
 from .sort_tokens import moe_sort_tokens, moe_unsort_tokens
-
-
-class _ExpertMLP(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, rows, gate_up_weight, down_weight, expert_offsets, act):
-        m, kept = glu_forward(product(rows, gate_up_weight, expert_offsets), act, True)
-        ctx.save_for_backward(rows if gate_up_weight.requires_grad else None, gate_up_weight, down_weight, expert_offsets, kept)
-        ctx.act = act
-        return product(m, down_weight, expert_offsets)
-
-    @staticmethod
-    @once
-    def backward(ctx, d_out):
-        rows, gate_up_weight, down_weight, offsets, kept = ctx.saved_tensors
-        want_rows, want_gate_up, want_down = ctx.needs_input_grad[:3]
-        d_out = tile_rows(d_out)
-        d_m = product(d_out, down_weight, offsets, transpose=True) if want_rows or want_gate_up else None
-        d_gate_up, m = glu_backward(d_m, kept, d_out.shape[0], down_weight.shape[1], ctx.act, want_m=want_down)
-        d_down = weight_grad(m, d_out, down_weight, offsets) if want_down else None
-        d_rows = product(d_gate_up, gate_up_weight, offsets, transpose=True) if want_rows else None
-        d_gate_up_weight = weight_grad(rows, d_gate_up, gate_up_weight, offsets) if want_gate_up else None
-        return d_rows, d_gate_up_weight, d_down, None, None
 
 
 def moe_expert_mlp(rows: torch.Tensor, gate_up_proj_weight: torch.Tensor, down_proj_weight: torch.Tensor,
@@ -55,11 +32,7 @@ def moe_expert_mlp(rows: torch.Tensor, gate_up_proj_weight: torch.Tensor, down_p
       2 * down_proj_weight.shape[1] == gate_up_proj_weight.shape[2], "down_proj_weight must be bfloat16 [E, I, H_out]")
     A(down_proj_weight.shape[1] % 8 == 0 and down_proj_weight.shape[2] % 8 == 0 and
       0 < down_proj_weight.shape[2] <= MOST_COLUMNS, "both sizes of down_proj_weight's matrices must be multiples of 8, at most 2^27")
-    act = activation_function.value
-    if needs_grad(rows, gate_up_proj_weight, down_proj_weight):
-        return _ExpertMLP.apply(rows, gate_up_proj_weight, down_proj_weight, expert_offsets, act)
-    m = glu_forward(product(rows, gate_up_proj_weight, expert_offsets), act, False)[0]
-    return product(m, down_proj_weight, expert_offsets)
+    return native().mlp(rows, gate_up_proj_weight, down_proj_weight, expert_offsets, activation_function.value)
 
 
 def moe_experts_train(hidden: torch.Tensor, affinities: torch.Tensor, expert_index: torch.Tensor,

@@ -8,56 +8,20 @@ import torch
 
 from .... import _lib
 from ...utils.common_types import ActFnType
-from .launch import MOST_ROWS, launch, needs_grad, once, pitch_of, refuse, tile_rows
+from .launch import MOST_ROWS, native, refuse
 
 _MOST_I = 2 ** 26
 
 
 def glu_forward(gate_up: torch.Tensor, act: int, keep: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``(m, kept)``; ``kept`` (the codes of all rows, then their scales) None unless ``keep``."""
-    R, two_I = gate_up.shape
-    I = two_I // 2
-    device = gate_up.device
-    m = torch.empty((R, I), dtype=torch.bfloat16, device=device)
-    kept = torch.empty(R * (two_I + 2 * ((I + 31) // 32)), dtype=torch.uint8, device=device) if keep else None
-    if R:
-        gate_up = tile_rows(gate_up)
-        codes = kept.data_ptr() if keep else None
-        launch(device, "b200moe_glu", gate_up.data_ptr(), pitch_of(gate_up), R, I, act, m.data_ptr(), codes,
-               codes + R * two_I if keep else None)
-    return m, kept
+    return native().glu_forward(gate_up, act, keep)
 
 
 def glu_backward(d_m: Optional[torch.Tensor], kept: torch.Tensor, R: int, I: int, act: int,
                  want_m: bool = False) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """``(d_gate_up, m)`` at the kept gate and up; the first None without ``d_m [R, I]``, the second unless wanted."""
-    device = kept.device
-    d_gate_up = None if d_m is None else torch.empty((R, 2 * I), dtype=torch.bfloat16, device=device)
-    m = torch.empty((R, I), dtype=torch.bfloat16, device=device) if want_m else None
-    if R:
-        pitch = I
-        if d_m is not None:
-            d_m = tile_rows(d_m)
-            pitch = pitch_of(d_m)
-        codes = kept.data_ptr()
-        launch(device, "b200moe_glu_backward", _lib.ptr(d_m), pitch, codes, codes + R * 2 * I, R, I, act, _lib.ptr(d_gate_up),
-               _lib.ptr(m))
-    return d_gate_up, m
-
-
-class _Glu(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, gate_up, act):
-        m, kept = glu_forward(gate_up, act, True)
-        ctx.save_for_backward(kept)
-        ctx.act = act
-        return m
-
-    @staticmethod
-    @once
-    def backward(ctx, d_m):
-        kept, = ctx.saved_tensors
-        return glu_backward(d_m, kept, *d_m.shape, ctx.act)[0], None
+    return native().glu_backward(d_m, kept, R, I, act, want_m)
 
 
 def moe_glu(gate_up: torch.Tensor, activation_function: ActFnType = ActFnType.SiLU) -> torch.Tensor:
@@ -80,6 +44,4 @@ def moe_glu(gate_up: torch.Tensor, activation_function: ActFnType = ActFnType.Si
         refuse(f"I must be a multiple of 8, gate_up has {gate_up.shape[1]} columns")
     if gate_up.shape[0] > MOST_ROWS or gate_up.shape[1] > 2 * _MOST_I:
         refuse(f"at most 2^30 rows of at most 2^27 columns, got {list(gate_up.shape)}")
-    if needs_grad(gate_up):
-        return _Glu.apply(gate_up, activation_function.value)
-    return glu_forward(gate_up, activation_function.value, False)[0]
+    return native().glu(gate_up, activation_function.value)

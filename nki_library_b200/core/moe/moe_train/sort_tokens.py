@@ -7,12 +7,11 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from .... import _lib
-from .launch import launch, needs_grad, once, pitch_of, refuse, same_device, unit_rows
+from .launch import native, refuse, same_device
 
 MAX_EXPERTS = 1024
 _ID_TYPES = (torch.int32, torch.uint32, torch.int64)
 _MOST_COLUMNS = 2 ** 30
-_ONE_LAUNCH = 2048  # pairs that the sort takes without a workspace
 
 
 class SortedTokens(NamedTuple):
@@ -26,7 +25,7 @@ class SortedTokens(NamedTuple):
     num_experts: int
 
 
-def _sort(expert_index: torch.Tensor, num_experts: int, hidden: Optional[torch.Tensor]):
+def _sort(hidden: Optional[torch.Tensor], expert_index: torch.Tensor, num_experts: int):
     """``(rows, plan)``; rows None without ``hidden``."""
     if not expert_index.is_cuda:
         _lib.require_cuda(expert_index)
@@ -37,39 +36,16 @@ def _sort(expert_index: torch.Tensor, num_experts: int, hidden: Optional[torch.T
     E = int(num_experts)
     if not 1 <= E <= MAX_EXPERTS:
         refuse(f"num_experts ({num_experts}) must be between 1 and {MAX_EXPERTS}")
-    T, K = expert_index.shape
-    pairs = T * K
-    if pairs >= 2 ** 31:
-        refuse(f"T * K ({pairs}) must be below 2^31")
-    device = expert_index.device
-    row_of_pair = torch.empty((T, K), dtype=torch.int32, device=device)
-    H = 0
-    rows = None
-    if hidden is not None:
-        H = hidden.shape[1]
-        rows = torch.empty((pairs, H), dtype=hidden.dtype, device=device)
-    if pairs == 0:
-        return rows, SortedTokens(torch.zeros(E + 1, dtype=torch.int32, device=device), row_of_pair, E)
-    index = expert_index.contiguous()
-    offsets = torch.empty(E + 1, dtype=torch.int32, device=device)
-    size, ws = 0, None
-    if pairs > _ONE_LAUNCH:
-        size = _lib.load_library().b200moe_sort_workspace_bytes(pairs, E)
-        ws = torch.empty(size, dtype=torch.uint8, device=device)
-    if H:
-        hidden = unit_rows(hidden)
-        launch(device, "b200moe_sort_tokens", hidden.data_ptr(), _lib.dtype_code(hidden), pitch_of(hidden), index.data_ptr(),
-               index.element_size(), T, K, H, E, offsets.data_ptr(), row_of_pair.data_ptr(), rows.data_ptr(), _lib.ptr(ws), size)
-    else:
-        launch(device, "b200moe_sort_pairs", index.data_ptr(), index.element_size(), T, K, E, offsets.data_ptr(),
-               row_of_pair.data_ptr(), _lib.ptr(ws), size)
+    if expert_index.numel() >= 2 ** 31:
+        refuse(f"T * K ({expert_index.numel()}) must be below 2^31")
+    rows, offsets, row_of_pair = native().sort(hidden, expert_index, E)
     return rows, SortedTokens(offsets, row_of_pair, E)
 
 
 def moe_sort_plan(expert_index: torch.Tensor, num_experts: int) -> SortedTokens:
     """Sort the pairs of ``expert_index [T, K]`` (int32, uint32 or int64).  Ids outside ``[0, num_experts)``, such as the -1
     of a dropped pair, get no row; equal ids of one token get a row each."""
-    return _sort(expert_index, num_experts, None)[1]
+    return _sort(None, expert_index, num_experts)[1]
 
 
 def _check_plan(plan: SortedTokens) -> Tuple[int, int]:
@@ -89,68 +65,6 @@ def _check_rows(t: torch.Tensor, name: str) -> None:
         refuse(f"{name} must have at most 2^30 columns")
 
 
-def _unsort_rows(rows: torch.Tensor, affinities: Optional[torch.Tensor], row_of_pair: torch.Tensor) -> torch.Tensor:
-    T, K = row_of_pair.shape
-    H = rows.shape[1]
-    if T * K * H == 0:
-        return torch.zeros((T, H), dtype=rows.dtype, device=rows.device)
-    out = torch.empty((T, H), dtype=rows.dtype, device=rows.device)
-    rows = unit_rows(rows)
-    if affinities is not None:
-        affinities = affinities.contiguous()
-    launch(rows.device, "b200moe_unsort_rows", rows.data_ptr(), _lib.dtype_code(rows), pitch_of(rows), T, K, H,
-           row_of_pair.data_ptr(), _lib.ptr(affinities), _lib.F32 if affinities is None else _lib.dtype_code(affinities),
-           out.data_ptr())
-    return out
-
-
-class _SortTokens(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, expert_index, num_experts):
-        rows, plan = _sort(expert_index, num_experts, hidden)
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(plan.expert_offsets, plan.row_of_pair)
-        ctx.save_for_backward(plan.row_of_pair)
-        return rows, plan.expert_offsets, plan.row_of_pair
-
-    @staticmethod
-    @once
-    def backward(ctx, d_rows, _offsets, _row_of_pair):
-        row_of_pair, = ctx.saved_tensors
-        return (None if d_rows is None else _unsort_rows(d_rows, None, row_of_pair)), None, None
-
-
-class _UnsortRows(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, rows, affinities, row_of_pair, expert_offsets):
-        # the rows are needed for the affinities' gradient only
-        ctx.save_for_backward(rows if affinities is not None and affinities.requires_grad else None, affinities, row_of_pair,
-                              expert_offsets)
-        return _unsort_rows(rows, affinities, row_of_pair)
-
-    @staticmethod
-    @once
-    def backward(ctx, d_out):
-        rows, affinities, row_of_pair, offsets = ctx.saved_tensors
-        T, K = row_of_pair.shape
-        H = d_out.shape[1]
-        want_rows, want_aff = ctx.needs_input_grad[:2]
-        d_rows = torch.empty((T * K, H), dtype=d_out.dtype, device=d_out.device) if want_rows else None
-        d_aff = torch.empty((T, K), dtype=affinities.dtype, device=d_out.device) if want_aff else None
-        if T * K * H == 0:
-            return d_rows, None if d_aff is None else d_aff.zero_(), None, None
-        d_out = unit_rows(d_out)
-        if want_aff:
-            rows = unit_rows(rows)
-        if affinities is not None:
-            affinities = affinities.contiguous()
-        launch(d_out.device, "b200moe_unsort_rows_backward", d_out.data_ptr(), pitch_of(d_out),
-               rows.data_ptr() if want_aff else None, pitch_of(rows) if want_aff else H, _lib.dtype_code(d_out), T, K, H,
-               offsets.numel() - 1, row_of_pair.data_ptr(), offsets.data_ptr(), _lib.ptr(affinities),
-               _lib.F32 if affinities is None else _lib.dtype_code(affinities), _lib.ptr(d_rows), _lib.ptr(d_aff))
-        return d_rows, d_aff, None, None
-
-
 def moe_sort_tokens(hidden: torch.Tensor, expert_index: torch.Tensor,
                     num_experts: int) -> Tuple[torch.Tensor, SortedTokens]:
     """Rows of ``hidden [T, H]`` (bf16 or fp32) sorted by expert: ``(rows [T * K, H], plan)``.
@@ -164,10 +78,7 @@ def moe_sort_tokens(hidden: torch.Tensor, expert_index: torch.Tensor,
     _check_rows(hidden, "hidden")
     if expert_index.dim() != 2 or expert_index.shape[0] != hidden.shape[0]:
         refuse("expert_index must be [T, K] with hidden's T")
-    if not needs_grad(hidden):
-        return _sort(expert_index, num_experts, hidden)
-    rows, offsets, row_of_pair = _SortTokens.apply(hidden, expert_index, num_experts)
-    return rows, SortedTokens(offsets, row_of_pair, int(num_experts))
+    return _sort(hidden, expert_index, num_experts)
 
 
 def moe_unsort_tokens(rows: torch.Tensor, affinities: Optional[torch.Tensor], plan: SortedTokens) -> torch.Tensor:
@@ -186,6 +97,4 @@ def moe_unsort_tokens(rows: torch.Tensor, affinities: Optional[torch.Tensor], pl
     if affinities is not None and (affinities.shape != plan.row_of_pair.shape or
                                    affinities.dtype not in (torch.float32, torch.bfloat16)):
         refuse(f"affinities must be [T, K] = [{T}, {K}], float32 or bfloat16")
-    if needs_grad(rows, affinities):
-        return _UnsortRows.apply(rows, affinities, plan.row_of_pair, plan.expert_offsets)
-    return _unsort_rows(rows, affinities, plan.row_of_pair)
+    return native().unsort(rows, affinities, plan.row_of_pair, plan.expert_offsets)

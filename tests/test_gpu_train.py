@@ -193,9 +193,12 @@ def test_rows_at_any_address(T, K, E, H, dtype):
     """Matrices anywhere between elements that are not theirs: NaN around every row that is read reaches no result, and what
     surrounds the rows that are written stays as it was."""
     from nki_library_b200 import _lib
-    from nki_library_b200.core.moe.moe_train.launch import launch
     import nki_library_b200 as m
     gen = _gen(T + H)
+
+    def launch(_device, name, *args):
+        _lib.call(name, *args, _lib.stream_ptr())
+
     idx = _ids(T, K, E, H, 0.1)
     plan = m.moe_sort_plan(idx, E)
     row, used = plan.row_of_pair, int(plan.expert_offsets[-1])
@@ -714,6 +717,40 @@ def test_second_derivatives_are_refused():
     first = torch.autograd.grad(out, leaves, d, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         first[0].float().sum().backward()
+
+
+@pytest.mark.parametrize("op", ["sort", "unsort", "linear", "glu", "mlp"])
+def test_losses_of_gradients_are_refused(op):
+    """A loss that holds an output and its gradient: what the gradient adds to the derivative would be missing, so it raises."""
+    import nki_library_b200 as m
+    idx, (hidden, aff, w1, w2), _ = _layer(2)
+    rows, plan = m.moe_sort_tokens(hidden, idx, w1.shape[0])
+    call, x = {
+        "sort": (lambda x: m.moe_sort_tokens(x, idx, w1.shape[0])[0], hidden),
+        "unsort": (lambda x: m.moe_unsort_tokens(x, aff, plan), rows),
+        "linear": (lambda x: m.expert_linear(x, w1, plan.expert_offsets), rows),
+        "glu": (lambda x: m.moe_glu(x), rows),
+        "mlp": (lambda x: m.moe_expert_mlp(x, w1, w2, plan.expert_offsets), rows),
+    }[op]
+    x = x.detach().requires_grad_()
+    out = call(x)
+    grad, = torch.autograd.grad(out.float().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (out.float().sum() + grad.float().square().sum()).backward()
+
+
+def test_errors_of_native_calls():
+    """What does not fit is torch's own error, and a refusal of an entry point is a refusal as everywhere; both leave all usable."""
+    import nki_library_b200 as m
+    from nki_library_b200.core.moe.moe_train.launch import native
+    one = torch.zeros(1, dtype=torch.bfloat16, device="cuda")
+    idx = torch.zeros((2 ** 20, 1), dtype=torch.int32, device="cuda")
+    with pytest.raises(torch.OutOfMemoryError):
+        m.moe_sort_tokens(one.expand(2 ** 20, 2 ** 20), idx, 1)
+    x = torch.zeros((4, 32), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(AssertionError, match="unknown activation"):
+        native().glu(x, 7)
+    assert not m.moe_glu(x).any()
 
 
 def test_captured_step_replays_on_new_inputs():
