@@ -120,3 +120,12 @@ def test_the_tests_rounding_agrees_with_the_types(I):
     cast = (v / s).to(torch.float8_e4m3fn).float() * s
     assert torch.equal(value.float()[finite], cast[finite]) and value[~finite].isnan().all()
     assert (torch.where(finite, (v / s).abs(), 0.0) <= 448).all()
+
+
+def test_native_part_is_built():
+    """Loads without a device, against the same library as everything else."""
+    from nki_library_b200.core.moe.moe_train.launch import native
+    part = native()
+    assert part.__file__.endswith("_autograd.so")
+    with pytest.raises(TypeError):
+        part.glu(None, 0)
