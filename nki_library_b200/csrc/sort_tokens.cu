@@ -276,7 +276,7 @@ __device__ __noinline__ uint2 careful(uintptr_t at, uintptr_t lo, uintptr_t hi) 
 // and last piece are cut, and a row that lies differently is read as the two or three aligned 8 bytes around each piece.  Sort,
 // sum with weights and its gradients of 16000 tokens x 7163 bf16, top-8: 408, 372, 755 us, and 694, 781, 1157 by 2 bytes at a
 // time; of 6000 x 5004, 8 experts: 112, 105, 203, and 143, 118, 230 by 4 bytes.  (Short rows of whole 4 bytes lose: 100000 x 130,
-// top-8 108, 106, 288 and 68, 141, 204.)
+// top-8 97, 106, 288 and 68, 141, 204.)
 template <typename T, bool WHOLE>
 struct Cut {
   // Column of piece p of the row at `row`; pieces with column >= H do not exist.
@@ -682,6 +682,17 @@ int check_sort(const void* expert_index, int index_bytes, int T, int K, int E, c
   return B200MOE_OK;
 }
 
+// bf16 rows of whole 4 bytes that are only copied are cut as fp32 ones of half the width, whose pieces have fewer ends (100000 x 130,
+// top-8: 97 us instead of 108; 16000 x 1002, top-4: 37.4 and 39.4).
+void widen_copy(int& dtype, int& H, int64_t& pitch, const void* from, const void* to) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to) |
+                         static_cast<uintptr_t>(H * 2) | static_cast<uintptr_t>(pitch * 2);
+  if (dtype != B200MOE_BF16 || bits % 4 != 0 || bits % 16 == 0) return;
+  dtype = B200MOE_F32;
+  H /= 2;
+  pitch /= 2;
+}
+
 // Calls fn with a value of the element type and whether all rows of the matrices are whole aligned 16 bytes, both known to the
 // compiler.
 template <typename F>
@@ -744,6 +755,7 @@ extern "C" int b200moe_sort_rows(const void* hidden, int dtype, int64_t pitch, i
   int rc = check_rows("sort_rows", dtype, T, K, H, pitch);
   if (rc != B200MOE_OK) return rc;
   B200MOE_REQUIRE(E > 0 && E <= kMaxExperts, B200MOE_ERR_INVALID, "sort_rows: between 1 and %d experts, got %d", kMaxExperts, E);
+  widen_copy(dtype, H, pitch, hidden, rows);
   const RowArgs a{T, K, H, E, row_of_pair, expert_offsets, T * K};
   return with_rows("sort_rows", dtype, H, {{hidden, pitch}, {rows, H}}, [&](auto element, auto whole) -> int {
     using T_ = decltype(element);
@@ -768,6 +780,7 @@ extern "C" int b200moe_sort_tokens(const void* hidden, int dtype, int64_t pitch,
   // One launch instead of two where a CTA per token does not repeat the order too often (16 tokens of 4096, 128 experts, top-8: 7.0 us
   // instead of 4.8 + 3.8, and 16.6 instead of 19.3 of host time)
   if (static_cast<int64_t>(T) * K <= kChunk && T <= 128) {
+    widen_copy(dtype, H, pitch, hidden, rows);
     const SortArgs s{expert_index, index_bytes == 8, static_cast<int64_t>(T) * K, E};
     const RowArgs a{T, K, H, E, nullptr, nullptr, T * K};
     return with_rows("sort_tokens", dtype, H, {{hidden, pitch}, {rows, H}}, [&](auto element, auto whole) -> int {
