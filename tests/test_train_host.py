@@ -129,3 +129,35 @@ def test_native_part_is_built():
     assert part.__file__.endswith("_autograd.so")
     with pytest.raises(TypeError):
         part.glu(None, 0)
+
+
+def _native_calls():
+    """The five operators on tensors, of the inputs that have a derivative: name -> (call, inputs)."""
+    from nki_library_b200.core.moe.moe_train.launch import native
+    op = native()
+    rows, weight = torch.zeros((8, 64), dtype=torch.bfloat16), torch.zeros((2, 64, 64), dtype=torch.bfloat16)
+    down = torch.zeros((2, 32, 64), dtype=torch.bfloat16)
+    idx, off = torch.zeros((4, 2), dtype=torch.int32), torch.tensor([0, 4, 8], dtype=torch.int32)
+    return {
+        "sort": (lambda x: op.sort(x, idx, 2), [rows[:4]]),
+        "unsort": (lambda x, a: op.unsort(x, a, idx, off), [rows, torch.zeros(4, 2)]),
+        "linear": (lambda x, w: op.linear(x, w, off, False), [rows, weight]),
+        "glu": (lambda x: op.glu(x, 0), [rows]),
+        "mlp": (lambda x, w, v: op.mlp(x, w, v, off, 0), [rows, weight, down]),
+    }
+
+
+OPERATORS = ["sort", "unsort", "linear", "glu", "mlp"]
+
+
+@pytest.mark.parametrize("op", OPERATORS)
+def test_dual_tensors_are_refused(op):
+    """A forward-mode tangent, on a tensor that asks for a gradient and on one that does not, of every input."""
+    import torch.autograd.forward_ad as forward
+    call, inputs = _native_calls()[op]
+    for i, x in enumerate(inputs):
+        for asks in (False, True):
+            with forward.dual_level():
+                dual = forward.make_dual(x.detach().requires_grad_(asks), torch.ones_like(x))
+                with pytest.raises(AssertionError, match="forward-mode"):
+                    call(*inputs[:i], dual, *inputs[i + 1:])
