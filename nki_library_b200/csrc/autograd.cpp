@@ -7,9 +7,11 @@
 #include <torch/extension.h>
 
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <memory>
 #include <optional>
@@ -70,9 +72,16 @@ bool recorded(std::initializer_list<Tensor> tensors) {
   return false;
 }
 
-// Forward-mode derivatives: a dual tensor need not ask for a gradient, so that the call would pass every node by and its result
-// come without a tangent, which reads as a derivative of zero.
-void refuse_duals(std::initializer_list<Tensor> tensors) {
+// What would take a launch for nothing.  Forward-mode derivatives: a dual tensor need not ask for a gradient, so that the call would
+// pass every node by and its result come without a tangent, which reads as a derivative of zero.  A recording of torch's calls: it
+// holds the allocation of a result and not the launch that fills it.
+bool recording() {
+  using c10::impl::TorchDispatchModeTLS;
+  return torch::jit::tracer::isTracing() ||
+         (TorchDispatchModeTLS::any_modes_set() && TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
+}
+void refuse_transforms(std::initializer_list<Tensor> tensors) {
+  if (recording()) throw EntryError("the training operators cannot be traced: a recording of torch's calls lacks their launches");
   for (const Tensor& t : tensors)
     if (t.defined() && t._fw_grad(0).defined())
       throw EntryError("the training operators have no forward-mode derivatives, neither of their results nor of their gradients");
@@ -140,7 +149,7 @@ struct SortTokens : torch::autograd::Function<SortTokens> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) {
     if (!d[0].defined()) return {Tensor(), Tensor(), Tensor()};
-    refuse_duals({d[0]});
+    refuse_transforms({d[0]});
     return once({unsort(d[0], Tensor(), ctx->get_saved_variables()[0]), Tensor(), Tensor()});
   }
 };
@@ -156,7 +165,7 @@ struct UnsortRows : torch::autograd::Function<UnsortRows> {
     return unsort(rows, affinities, row_of_pair);
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) {
-    refuse_duals({d[0]});
+    refuse_transforms({d[0]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &affinities = saved[1], &row_of_pair = saved[2], &offsets = saved[3];
     const On on(d[0]);
@@ -253,7 +262,7 @@ struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
     return product(rows, weight, offsets, false, check_status);
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) {
-    refuse_duals({d[0]});
+    refuse_transforms({d[0]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor d_out = tile_rows(d[0]);
     Tensor d_rows, d_weight;
@@ -303,7 +312,7 @@ struct Glu : torch::autograd::Function<Glu> {
     return m;
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) {
-    refuse_duals({d[0]});
+    refuse_transforms({d[0]});
     const Tensor kept = ctx->get_saved_variables()[0];
     return once({std::get<0>(glu_backward(d[0], kept, d[0].size(0), d[0].size(1), ctx->saved_data["act"].toInt(), false)), Tensor()});
   }
@@ -319,7 +328,7 @@ struct ExpertMLP : torch::autograd::Function<ExpertMLP> {
     return product(m, down_weight, offsets, false, false);
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) {
-    refuse_duals({d[0]});
+    refuse_transforms({d[0]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &rows = saved[0], &gate_up_weight = saved[1], &down_weight = saved[2], &offsets = saved[3];
     const bool want_rows = ctx->needs_input_grad(0), want_gate_up = ctx->needs_input_grad(1), want_down = ctx->needs_input_grad(2);
@@ -340,7 +349,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, module) {
   // every exception the way torch's own calls raise it (out of memory, refusals)
   const auto def = [&](const char* name, auto&& f) { module.def(name, torch::wrap_pybind_function(f)); };
   def("sort", [](const Maybe& hidden, const Tensor& index, int64_t E) -> std::tuple<Maybe, Tensor, Tensor> {
-    refuse_duals({or_none(hidden)});
+    refuse_transforms({or_none(hidden)});
     if (hidden.has_value() && recorded({*hidden})) {
       const variable_list out = SortTokens::apply(*hidden, index, E);
       return {out[0], out[1], out[2]};
@@ -349,22 +358,22 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, module) {
     return {maybe(rows), offsets, row_of_pair};
   });
   def("unsort", [](const Tensor& rows, const Maybe& affinities, const Tensor& row_of_pair, const Tensor& offsets) {
-    refuse_duals({rows, or_none(affinities)});
+    refuse_transforms({rows, or_none(affinities)});
     if (recorded({rows, or_none(affinities)})) return UnsortRows::apply(rows, affinities, row_of_pair, offsets);
     return unsort(rows, or_none(affinities), row_of_pair);
   });
   def("linear", [](const Tensor& rows, const Tensor& weight, const Tensor& offsets, bool check_status) {
-    refuse_duals({rows, weight});
+    refuse_transforms({rows, weight});
     return recorded({rows, weight}) ? ExpertLinear::apply(rows, weight, offsets, check_status)
                                     : product(rows, weight, offsets, false, check_status);
   });
   def("glu", [](const Tensor& gate_up, int64_t act) {
-    refuse_duals({gate_up});
+    refuse_transforms({gate_up});
     return recorded({gate_up}) ? Glu::apply(gate_up, act) : std::get<0>(glu_forward(gate_up, act, false));
   });
   def("mlp", [](const Tensor& rows, const Tensor& gate_up_weight, const Tensor& down_weight, const Tensor& offsets,
                        int64_t act) {
-    refuse_duals({rows, gate_up_weight, down_weight});
+    refuse_transforms({rows, gate_up_weight, down_weight});
     if (recorded({rows, gate_up_weight, down_weight})) return ExpertMLP::apply(rows, gate_up_weight, down_weight, offsets, act);
     const Tensor m = std::get<0>(glu_forward(product(rows, gate_up_weight, offsets, false, false), act, false));
     return product(m, down_weight, offsets, false, false);

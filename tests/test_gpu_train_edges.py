@@ -43,3 +43,18 @@ def test_forward_mode_is_refused(op):
     with pytest.raises(Exception):
         torch.func.jvp(call, (x,), (torch.ones_like(x),))
     assert torch.autograd.grad(out, leaf, torch.ones_like(out))[0].shape == x.shape
+
+
+@pytest.mark.parametrize("op", OPERATORS)
+def test_tracing_is_refused(op):
+    """In the operator and in its backward pass; outside, both go on as before."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, x = _operator(op)
+    leaf = x.clone().requires_grad_()
+    out = call(leaf)
+    for trace in (lambda f, y: torch.jit.trace(f, y), lambda f, y: make_fx(f)(y)):
+        with pytest.raises(AssertionError, match="cannot be traced"):
+            trace(lambda y: call(y), x)
+    with pytest.raises(AssertionError, match="cannot be traced"):
+        make_fx(lambda d: torch.autograd.grad(out, leaf, d, retain_graph=True)[0])(torch.ones_like(out))
+    assert torch.equal(call(x), out) and torch.autograd.grad(out, leaf, torch.ones_like(out))[0].shape == x.shape

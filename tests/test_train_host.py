@@ -161,3 +161,14 @@ def test_dual_tensors_are_refused(op):
                 dual = forward.make_dual(x.detach().requires_grad_(asks), torch.ones_like(x))
                 with pytest.raises(AssertionError, match="forward-mode"):
                     call(*inputs[:i], dual, *inputs[i + 1:])
+
+
+@pytest.mark.parametrize("op", OPERATORS)
+def test_tracing_is_refused(op):
+    """A recorded call would hold the allocation of its result and no launch, and replay memory that nothing has filled."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, inputs = _native_calls()[op]
+    with pytest.raises(AssertionError, match="cannot be traced"):
+        torch.jit.trace(call, tuple(inputs))
+    with pytest.raises(AssertionError, match="cannot be traced"):
+        make_fx(call)(*inputs)
