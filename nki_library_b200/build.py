@@ -59,7 +59,34 @@ def _autograd_link(target: str) -> list:
             "-Wl,-rpath,$ORIGIN"]
 
 
+def _report(command: list, out: str, verbose: bool, failed: bool) -> None:
+    if failed or verbose:
+        sys.stderr.write(out or " ".join(command) + "\n")
+
+
+def _start_autograd(hdr: str, force: bool):
+    """The running compiler of the torch side, None if there is nothing to compile."""
+    source, obj = os.path.join(CSRC, "autograd.cpp"), os.path.join(BUILD, "autograd.o")
+    if not (force or _stale(obj, [source, hdr])):
+        return None
+    return subprocess.Popen(_autograd_compile(source, obj), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+
+
+def _finish_autograd(compiler, force: bool, verbose: bool) -> None:
+    obj = os.path.join(BUILD, "autograd.o")
+    if compiler is not None:
+        out, _ = compiler.communicate()
+        _report(compiler.args, out, verbose, compiler.returncode != 0)
+        if compiler.returncode != 0:
+            raise RuntimeError("compilation failed")
+    if force or _stale(AUTOGRAD, [obj]):
+        subprocess.check_call(_autograd_link(obj))
+
+
 def build_library(force: bool = False, verbose: bool = False) -> str:
+    """The shared library; raises if it cannot be built.  The torch side is built beside it where torch is installed.  A C program
+    needs neither, so what goes wrong there (no Python headers, a torch without CUDA) is reported and leaves the library as it is;
+    the training operators then raise on their first call."""
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
     hdrs = sorted(glob.glob(os.path.join(CSRC, "*.cuh"))) + [os.path.join(os.path.dirname(PKG), "include", "b200moe.h")]
     os.makedirs(BUILD, exist_ok=True)
@@ -70,24 +97,35 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
         objs.append(o)
         if force or _stale(o, [s] + hdrs):
             cmd = [_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", s, "-o", o]
-            procs.append((s, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
-    source, autograd = os.path.join(CSRC, "autograd.cpp"), os.path.join(BUILD, "autograd.o")
-    torch = importlib.util.find_spec("torch") is not None  # a C program needs neither it nor this part
-    if torch and (force or _stale(autograd, [source, hdrs[-1]])):
-        procs.append((source, subprocess.Popen(_autograd_compile(source, autograd), stdout=subprocess.PIPE,
-                                               stderr=subprocess.STDOUT, text=True)))
+            procs.append(subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
+    torch_side, trouble = None, None
+    if importlib.util.find_spec("torch") is not None:
+        try:
+            torch_side = _start_autograd(hdrs[-1], force)
+        except Exception as error:
+            trouble = error
+    else:
+        trouble = "torch is not installed"
     failed = False
-    for s, p in procs:
+    for p in procs:
         out, _ = p.communicate()
-        if p.returncode != 0 or verbose:
-            sys.stderr.write(out)
+        _report(p.args, out, verbose, p.returncode != 0)
         failed |= p.returncode != 0
     if failed:
+        if torch_side is not None:
+            torch_side.communicate()
         raise RuntimeError("compilation failed")
     if force or procs or _stale(LIB, objs):
         subprocess.check_call([_nvcc(), "-shared", "-o", LIB] + objs + ["-lcudart"])
-    if torch and (force or _stale(AUTOGRAD, [autograd])):
-        subprocess.check_call(_autograd_link(autograd))
+    try:
+        if trouble is None:
+            _finish_autograd(torch_side, force, verbose)
+    except Exception as error:
+        trouble = error
+    if trouble is not None:
+        if os.path.exists(AUTOGRAD):  # it would fit an earlier library
+            os.remove(AUTOGRAD)
+        sys.stderr.write(f"{LIB} is built; {AUTOGRAD}, which the training operators need, is not: {trouble}\n")
     return LIB
 
 
