@@ -64,9 +64,28 @@ def _report(command: list, out: str, verbose: bool, failed: bool) -> None:
         sys.stderr.write(out or " ".join(command) + "\n")
 
 
+def _write_stamp() -> bool:
+    """Names the torch and the Python that the torch side is compiled against beside it; whether these are others than before."""
+    import sysconfig
+
+    import torch
+
+    path = os.path.join(BUILD, "autograd.stamp")
+    text = f"{torch.__version__} {os.path.dirname(torch.__file__)} {sysconfig.get_config_var('SOABI')}\n"
+    if os.path.exists(path):
+        with open(path) as f:
+            if f.read() == text:
+                return False
+    with open(path, "w") as f:
+        f.write(text)
+    return True
+
+
 def _start_autograd(hdr: str, force: bool):
     """The running compiler of the torch side, None if there is nothing to compile."""
     source, obj = os.path.join(CSRC, "autograd.cpp"), os.path.join(BUILD, "autograd.o")
+    if _write_stamp() and os.path.exists(obj):
+        os.remove(obj)
     if not (force or _stale(obj, [source, hdr])):
         return None
     return subprocess.Popen(_autograd_compile(source, obj), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)

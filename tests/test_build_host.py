@@ -52,3 +52,20 @@ def test_a_library_that_does_not_compile_raises(build):
         f.write("#error not this one\n")
     with pytest.raises(RuntimeError, match="compilation failed"):
         build.build_library()
+
+
+def test_another_torch_rebuilds_the_torch_side(build, monkeypatch):
+    """Also where the build in between failed."""
+    import torch
+    build.build_library()
+    first = os.stat(build.AUTOGRAD).st_mtime_ns
+    build.build_library()
+    assert os.stat(build.AUTOGRAD).st_mtime_ns == first
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    compile_ = build._autograd_compile
+    monkeypatch.setattr(build, "_autograd_compile", lambda source, target: ["false"])
+    build.build_library()
+    assert not os.path.exists(build.AUTOGRAD)
+    monkeypatch.setattr(build, "_autograd_compile", compile_)
+    build.build_library()
+    assert os.stat(build.AUTOGRAD).st_mtime_ns > first
