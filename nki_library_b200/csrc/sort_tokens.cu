@@ -661,7 +661,7 @@ Layout row_layout(int T, int H, int per_thread, int threads, bool spread) {
   }
   const int x = lanes <= threads / 4 ? (lanes <= 32 ? 32 : threads / 4) : (lanes <= threads / 2 ? threads / 2 : threads);
   const int y = threads / x;
-  return {dim3((T + y - 1) / y), dim3(x, y)};
+  return {dim3(static_cast<unsigned>(ceil_div64(T, y))), dim3(x, y)};
 }
 
 int check_rows(const char* name, int dtype, int T, int K, int H, int64_t pitch) {

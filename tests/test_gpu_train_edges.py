@@ -58,3 +58,29 @@ def test_tracing_is_refused(op):
     with pytest.raises(AssertionError, match="cannot be traced"):
         make_fx(lambda d: torch.autograd.grad(out, leaf, d, retain_graph=True)[0])(torch.ones_like(out))
     assert torch.equal(call(x), out) and torch.autograd.grad(out, leaf, torch.ones_like(out))[0].shape == x.shape
+
+
+def test_the_most_tokens():
+    """2^31 - 1 tokens of one column: sorted, summed and back through both gradients."""
+    import nki_library_b200 as m
+    T = 2 ** 31 - 1
+    hidden = torch.ones((1, 1), dtype=torch.bfloat16, device="cuda").expand(T, 1).contiguous()
+    hidden[-1] = 2
+    idx = torch.zeros((T, 1), dtype=torch.int32, device="cuda")
+    idx[0], idx[-2] = -1, 1
+    rows, plan = m.moe_sort_tokens(hidden, idx, 2)
+    assert plan.expert_offsets.tolist() == [0, T - 2, T - 1]
+    row = plan.row_of_pair.view(-1)
+    ends = {0: -1, 1: 0, T // 2: T // 2 - 1, T - 3: T - 4, T - 2: T - 2, T - 1: T - 3}  # token: its row
+    assert [int(row[t]) for t in ends] == list(ends.values())
+    step = 1 << 28
+    for lo in range(1, T - 2, step):
+        hi = min(lo + step, T - 2)
+        assert torch.equal(row[lo:hi], torch.arange(lo - 1, hi - 1, dtype=torch.int32, device="cuda"))
+    assert rows[T - 3] == 2 and rows[T - 1] == 0 and int((rows == 1).sum()) == T - 2
+    del idx
+    rows.requires_grad_()
+    out = m.moe_unsort_tokens(rows, None, plan)
+    assert out[0] == 0 and out[-1] == 2 and int((out == 1).sum()) == T - 2
+    d_rows, = torch.autograd.grad(out, rows, hidden)
+    assert d_rows[T - 3] == 2 and d_rows[T - 1] == 0 and int((d_rows == 1).sum()) == T - 2
