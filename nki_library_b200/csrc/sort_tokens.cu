@@ -684,10 +684,14 @@ int check_sort(const void* expert_index, int index_bytes, int T, int K, int E, c
 
 // bf16 rows of whole 4 bytes that are only copied are cut as fp32 ones of half the width, whose pieces have fewer ends (100000 x 130,
 // top-8: 97 us instead of 108; 16000 x 1002, top-4: 37.4 and 39.4).
+// H may be 2^30, whose bytes pass 32 bits.
+constexpr bool copied_as_fp32(uint64_t addresses, int H, int64_t pitch) {
+  const uint64_t bits = addresses | (static_cast<uint64_t>(H) * 2) | (static_cast<uint64_t>(pitch) * 2);
+  return bits % 4 == 0 && bits % 16 != 0;
+}
+static_assert(copied_as_fp32(4, 1 << 30, int64_t{1} << 30) && !copied_as_fp32(16, 1 << 30, int64_t{1} << 30) && !copied_as_fp32(2, 8, 8));
 void widen_copy(int& dtype, int& H, int64_t& pitch, const void* from, const void* to) {
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to) |
-                         static_cast<uintptr_t>(H * 2) | static_cast<uintptr_t>(pitch * 2);
-  if (dtype != B200MOE_BF16 || bits % 4 != 0 || bits % 16 == 0) return;
+  if (dtype != B200MOE_BF16 || !copied_as_fp32(reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to), H, pitch)) return;
   dtype = B200MOE_F32;
   H /= 2;
   pitch /= 2;

@@ -84,3 +84,17 @@ def test_the_most_tokens():
     assert out[0] == 0 and out[-1] == 2 and int((out == 1).sum()) == T - 2
     d_rows, = torch.autograd.grad(out, rows, hidden)
     assert d_rows[T - 3] == 2 and d_rows[T - 1] == 0 and int((d_rows == 1).sum()) == T - 2
+
+
+def test_the_widest_rows():
+    """2^30 columns of bf16, 4 bytes off a 16-byte boundary: copied as fp32 rows of half the width."""
+    from nki_library_b200 import _lib
+    H = 2 ** 30
+    flat = torch.arange(2 ** 15, dtype=torch.int32, device="cuda").to(torch.int16).repeat(H // 2 ** 15 + 1).view(torch.bfloat16)
+    hidden, out = flat[2:2 + H], torch.zeros(H + 8, dtype=torch.bfloat16, device="cuda")
+    idx = torch.zeros(1, dtype=torch.int32, device="cuda")
+    offsets, row = torch.empty(2, dtype=torch.int32, device="cuda"), torch.empty(1, dtype=torch.int32, device="cuda")
+    _lib.call("b200moe_sort_tokens", hidden.data_ptr(), _lib.BF16, H, idx.data_ptr(), 4, 1, 1, H, 1, offsets.data_ptr(), row.data_ptr(),
+              out[2:].data_ptr(), None, 0, _lib.stream_ptr())
+    assert torch.equal(out[2:2 + H].view(torch.int16), hidden.view(torch.int16)) and not out[:2].any() and not out[2 + H:].any()
+    assert offsets.tolist() == [0, 1] and row.tolist() == [0]
