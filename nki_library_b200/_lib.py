@@ -121,6 +121,7 @@ SIGNATURES = {
     "b200moe_expert_product_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "b200moe_expert_product": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int, c_int,
                                        c_int, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "b200moe_expert_wait_cycles": (c_int64, [c_int64]),
     "b200moe_expert_weight_grad_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "b200moe_expert_weight_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int,
                                            c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),

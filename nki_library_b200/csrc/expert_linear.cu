@@ -27,9 +27,11 @@
 //          the 32 values a warp holds of a row are 64 contiguous bytes and go straight out.  Turning a chunk around in
 //          shared memory for longer stores costs the tensor pipe operand bandwidth, which the ring's copies and the MMAs
 //          use up (4 x 1024 rows, 4096 x 14336, weight grad: 361 us turned, 353 straight; 32 x 16 rows, 4096 x 4096: 248, 194).
-// Every wait is bounded; on expiry a code goes to `status`, no more work is issued and the kernel tears down.
+// Every wait is bounded; on expiry a code goes to `status`, no more work is issued and the kernel tears down, behind the copies and
+// MMAs that are under way.
 #include <cuda.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -74,6 +76,7 @@ struct Params {
   float* partial;    // [parts][output rows][cols]
   int64_t out_rows;  // of all experts
   int32_t* status;
+  int64_t wait_cycles;  // a wait gives up after as many
   int32_t* taken;  // tiles handed out beyond every pair's first; NULL: pair u walks tiles u, u + pairs, ...
   int queue;       // ... and how many of them a pair holds at most
 };
@@ -125,17 +128,36 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t pa
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* status,
-                                                  int code) {
-  const long long t0 = clock64();
-  while (!mbar_try_wait_cluster(bar, parity)) {
-    if (*abort_flag) return false;
-    if (clock64() - t0 > kWaitCycles) {
-      *abort_flag = 1;
-      atomicCAS(status, 0, code);
-      return false;
-    }
+// A wait's bound and where it is reported.
+struct Bound {
+  volatile int* abort_flag;  // of the CTA
+  int32_t* status;
+  int64_t cycles;
+  // Whether a wait that began at t0 is over without its barrier: its time is up or another warp of the CTA has given up.
+  __device__ __forceinline__ bool over(long long t0, int code) const {
+    if (*abort_flag) return true;
+    if (clock64() - t0 <= cycles) return false;
+    *abort_flag = 1;
+    atomicCAS(status, 0, code);
+    return true;
   }
+};
+// A whole warp waits.  Its lanes leave together: one that saw the barrier complete beside one that saw the CTA give up would wait
+// for it at the next __syncwarp for good.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Bound& bound, int code) {
+  const auto done = [&] { return __all_sync(0xffffffffu, CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)); };
+  if (done()) return true;
+  const long long t0 = clock64();
+  while (!done())
+    if (__any_sync(0xffffffffu, bound.over(t0, code))) return false;
+  return true;
+}
+// One lane waits, the others do not.
+__device__ __forceinline__ bool lane_wait_cluster(uint64_t* bar, uint32_t parity, const Bound& bound, int code) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait_cluster(bar, parity))
+    if (bound.over(t0, code)) return false;
   return true;
 }
 
@@ -227,7 +249,7 @@ struct Walk {
   const Params& p;
   const Sched& s;
   uint64_t *full, *empty;  // of the queue's entries: per CTA, in the odd CTA
-  volatile int* abort_flag;
+  const Bound& bound;
   int unit, n_units, total, i;
   // The next tile, -1 behind the last.
   __device__ __forceinline__ int next() {
@@ -237,7 +259,7 @@ struct Walk {
       return tile < total ? static_cast<int>(tile) : -1;
     }
     const int slot = (at - 1) % p.queue;
-    if (!mbar_wait_cluster(&full[slot], (at - 1) / p.queue & 1, abort_flag, p.status, 47)) return -1;
+    if (!warp_wait<true>(&full[slot], (at - 1) / p.queue & 1, bound, 47)) return -1;
     const int tile = *static_cast<const volatile int*>(&s.queue[slot]);
     __syncwarp();
     if (tile >= total) return -1;
@@ -344,7 +366,8 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr;
   const int total = (WGRAD ? p.E * p.row_tiles * p.col_tiles : s.tiles[p.E]) * p.parts;
-  Walk<!WGRAD> walk{p, s, queue_full, queue_empty, abort_flag, unit, n_units, total, 0};
+  const Bound bound{abort_flag, p.status, p.wait_cycles};
+  Walk<!WGRAD> walk{p, s, queue_full, queue_empty, bound, unit, n_units, total, 0};
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer of the column operand
@@ -358,7 +381,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
       // the even CTA's barrier counts both CTAs' bytes
       const uint32_t bytes = 2 * kOperand + (WGRAD ? (t.rows > 128 ? 2 : 1) * kOperand : round_up32(t.rows) * 128);
       for (int kb = 0; kb < slabs; ++kb) {
-        if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, 41)) { ok = false; break; }
+        if (!warp_wait(&empty[stage], phase ^ 1u, bound, 41)) { ok = false; break; }
         uint8_t* dst = smem + stage * kStage;
         if (leader) {
           if (rank == 0) mbar_expect_tx(&full[stage], bytes);
@@ -375,10 +398,6 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
         if (++stage == kStages) { stage = 0; phase ^= 1u; }
       }
     }
-    if (!ok) {
-      // let copies already in flight land before the CTA retires
-      for (int i = 0; i < 2000; ++i) __nanosleep(1000);
-    }
   } else if (warp == 3) {
     // ------------------------------------------------------------ producer of the row operand
     const bool leader = elect_one();
@@ -391,7 +410,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
       const int half = round_up32(t.rows) >> 1;
       const int r = t.row0 + rank * half;
       for (int kb = 0; kb < slabs; ++kb) {
-        if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, 41)) { ok = false; break; }
+        if (!warp_wait(&empty[stage], phase ^ 1u, bound, 41)) { ok = false; break; }
         uint8_t* dst = smem + stage * kStage + kOperand;
         if (leader) {
           if constexpr (WGRAD) {
@@ -408,9 +427,6 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
         }
         if (++stage == kStages) { stage = 0; phase ^= 1u; }
       }
-    }
-    if (!ok) {
-      for (int i = 0; i < 2000; ++i) __nanosleep(1000);
     }
   } else if (warp == 1 && rank == 0) {
     // ------------------------------------------------------------ MMA issuer
@@ -431,11 +447,11 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
       if (slabs == 0) advance();
       if (WGRAD && k == 0) continue;
       const int acc = it & 1;
-      if (!mbar_wait(&tmem_empty[acc], ((it >> 1) & 1) ^ 1u, abort_flag, p.status, 42)) break;
+      if (!warp_wait(&tmem_empty[acc], ((it >> 1) & 1) ^ 1u, bound, 42)) break;
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + acc * 256;
       for (int kb = 0; kb < slabs; ++kb) {
-        if (!mbar_wait(&full[stage], phase, abort_flag, p.status, 43)) { ok = false; break; }
+        if (!warp_wait(&full[stage], phase, bound, 43)) { ok = false; break; }
         tc_fence_after();
         const uint32_t sc = smem_u32(smem + stage * kStage), sr = sc + kOperand;
         const uint64_t c_desc = COL_MN ? desc_sw128_mn(sc) : desc_sw128(sc);
@@ -454,7 +470,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
       }
       if constexpr (WGRAD) if (ok && (k & 15) != 0) {
         const int b = ends % C::kTails;
-        if (!mbar_wait_cluster(&tail_ready[b], ends / C::kTails & 1, abort_flag, p.status, 44)) break;
+        if (!warp_wait<true>(&tail_ready[b], ends / C::kTails & 1, bound, 44)) break;
         tc_fence_after();
         const uint32_t sc = smem_u32(smem + C::kOffTail + b * kTail);
         if (leader) {
@@ -471,7 +487,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
     if (!WGRAD && p.taken != nullptr && lane == 0) {
       for (int i = 0, tile = 0; tile < total; ++i) {
         const int slot = i % p.queue;
-        if (!mbar_wait_cluster(&queue_empty[slot], (i / p.queue & 1) ^ 1u, abort_flag, p.status, 48)) break;
+        if (!lane_wait_cluster(&queue_empty[slot], (i / p.queue & 1) ^ 1u, bound, 48)) break;
         tile = n_units + atomicAdd(p.taken, 1);
         *static_cast<volatile int*>(&s.queue[slot]) = tile;
         uint32_t remote;
@@ -501,7 +517,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
       if (rest == 0) continue;
       const int b = ends % C::kTails;
       uint8_t* base = smem + C::kOffTail + b * kTail;
-      if (!mbar_wait(&tail_full[b], ends / C::kTails & 1, abort_flag, p.status, 45)) break;
+      if (!warp_wait(&tail_full[b], ends / C::kTails & 1, bound, 45)) break;
       // 32 lanes clear 512 bytes: a row of all four boxes
       for (int r = rest; r < 16; ++r)
         *reinterpret_cast<uint4*>(base + (lane >> 3) * 2048 + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -521,10 +537,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
       if ((t.k & 15) == 0) continue;
       const int b = ends % C::kTails;
       uint8_t* base = smem + C::kOffTail + b * kTail;
-      if (!mbar_wait(&tail_empty[b], (ends / C::kTails & 1) ^ 1u, abort_flag, p.status, 49)) {
-        for (int i = 0; i < 2000; ++i) __nanosleep(1000);
-        break;
-      }
+      if (!warp_wait(&tail_empty[b], (ends / C::kTails & 1) ^ 1u, bound, 49)) break;
       if (leader) {
         const int c = t.c0 + rank * 128, r = t.row0 + rank * (round_up32(t.rows) >> 1), k = t.k0 + (t.k & ~15);
         mbar_expect_tx(&tail_full[b], kTail);
@@ -557,7 +570,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
       }
       const int col = t.c0 + rank * 128 + q * 32 + lane;
       const int acc = it & 1;
-      if (!mbar_wait(&tmem_full[acc], (it >> 1) & 1, abort_flag, p.status, 46)) break;
+      if (!warp_wait(&tmem_full[acc], (it >> 1) & 1, bound, 46)) break;
       __syncwarp();
       tc_fence_after();
       ++it;
@@ -600,6 +613,11 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
 
   tc_fence_before();
   __syncthreads();
+  // A pair that has given up may have copies and MMAs under way whose end nothing awaits, of microseconds: they get a hundred times
+  // that before shared memory and TMEM go.  (A CTA whose waits all came through has none of its own.)
+  if (*abort_flag)
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  __syncwarp();
   cluster_sync_all();  // the peer may still read this CTA's shared memory until here
   if (warp == 1) {
     tc_fence_after();
@@ -697,6 +715,8 @@ int launch(const CUtensorMap& cols, const RowMaps& rows, const Params& p, int64_
   return B200MOE_OK;
 }
 
+std::atomic<int64_t> wait_cycles{kWaitCycles};
+
 bool rows_ok(const void* p, int64_t pitch, int cols) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && pitch % 8 == 0 && pitch >= cols && pitch < (int64_t{1} << 38);
 }
@@ -705,6 +725,8 @@ bool rows_ok(const void* p, int64_t pitch, int cols) {
 }  // namespace b200moe
 
 using namespace b200moe;
+
+extern "C" int64_t b200moe_expert_wait_cycles(int64_t cycles) { return wait_cycles.exchange(cycles); }
 
 extern "C" size_t b200moe_expert_product_workspace_bytes(int contract_last, int R, int E, int D0, int D1) {
   if (R <= 0 || E <= 0 || D0 <= 0 || D1 <= 0) return 0;
@@ -745,6 +767,7 @@ extern "C" int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch,
   p.per_matrix = p.per_group = make_divisor(static_cast<uint32_t>(kGroup * p.col_tiles));
   p.out = static_cast<__nv_bfloat16*>(out_bf16);
   p.status = status;
+  p.wait_cycles = wait_cycles.load();
   const int64_t most_tiles = product_tiles(R, E, n);
   p.parts = split_parts(most_tiles, ceil_div64(k, 64));
   p.partial = static_cast<float*>(workspace);
@@ -804,6 +827,7 @@ extern "C" int b200moe_expert_weight_grad(const void* a_bf16, int64_t a_pitch, c
   p.width = ((M + p.row_tiles - 1) / p.row_tiles + 31) & ~31;
   p.out = static_cast<__nv_bfloat16*>(out_bf16);
   p.status = status;
+  p.wait_cycles = wait_cycles.load();
   const int64_t tiles = weight_grad_tiles(E, M, N);
   p.parts = split_parts(tiles, R / (static_cast<int64_t>(E) * 64));
   p.partial = static_cast<float*>(workspace);

@@ -1,5 +1,7 @@
 """Calls of the experts' training pass that have to be refused, reported or answered at the ends of their ranges."""
 
+import contextlib
+
 import pytest
 import torch
 
@@ -98,3 +100,68 @@ def test_the_widest_rows():
               out[2:].data_ptr(), None, 0, _lib.stream_ptr())
     assert torch.equal(out[2:2 + H].view(torch.int16), hidden.view(torch.int16)) and not out[:2].any() and not out[2 + H:].any()
     assert offsets.tolist() == [0, 1] and row.tolist() == [0]
+
+
+# ------------------------------------------------------------------ waits that run out
+@contextlib.contextmanager
+def _wait_cycles(cycles):
+    """Products launched inside give up a wait after `cycles` clocks; below zero at the first look that finds it unfinished."""
+    from nki_library_b200 import _lib
+    lib = _lib.load_library()
+    before = lib.b200moe_expert_wait_cycles(cycles)
+    try:
+        yield
+    finally:
+        assert lib.b200moe_expert_wait_cycles(before) == cycles
+
+
+class _Product:
+    """A product or a weight gradient through the C entry points."""
+
+    def __init__(self, counts, K, N, weight_grad=False, behind=0):
+        gen = torch.Generator(device="cuda").manual_seed(K + N)
+        self.E, self.R, self.K, self.N, self.weight_grad = len(counts), sum(counts) + behind, K, N, weight_grad
+        self.offsets = torch.tensor([0] + counts).cumsum(0).int().cuda()
+        self.x = torch.randint(-2, 3, (self.R, K), device="cuda", generator=gen).bfloat16()
+        other = (self.R, N) if weight_grad else (self.E, K, N)
+        self.w = torch.randint(-2, 3, other, device="cuda", generator=gen).bfloat16()
+
+    def run(self):
+        """(output, status)"""
+        from nki_library_b200 import _lib
+        lib = _lib.load_library()
+        E, R, K, N = self.E, self.R, self.K, self.N
+        out = torch.zeros((E, K, N) if self.weight_grad else (R, N), dtype=torch.bfloat16, device="cuda")
+        status = torch.full((2,), -1, dtype=torch.int32, device="cuda")
+        if self.weight_grad:
+            size = lib.b200moe_expert_weight_grad_workspace_bytes(R, E, K, N)
+            ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+            _lib.call("b200moe_expert_weight_grad", self.x.data_ptr(), K, self.w.data_ptr(), N, self.offsets.data_ptr(), R, E, K, N,
+                      out.data_ptr(), ws.data_ptr(), size, status.data_ptr(), _lib.stream_ptr())
+        else:
+            size = lib.b200moe_expert_product_workspace_bytes(0, R, E, K, N)
+            ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+            _lib.call("b200moe_expert_product", self.x.data_ptr(), K, self.w.data_ptr(), N, K * N, 0, self.offsets.data_ptr(), R, E, K, N,
+                      out.data_ptr(), ws.data_ptr(), size, status.data_ptr(), _lib.stream_ptr())
+        torch.cuda.synchronize()
+        return out, int(status[0])
+
+
+# Contractions of 1024 slabs and more in one tile each, which an accumulator's readers wait for longer than one look lasts (20 us): one
+# tile per pair, tiles handed out, a weight gradient with ragged ends, parts of a contraction, parts of a weight gradient.
+LONG = [([3] * 40, 65536, 8, False, 0), ([8192], 65536, 8192, False, 3), ([70001] + [1] * 39, 8, 8, True, 0), ([5, 2], 2 ** 21, 16, False, 1),
+        ([2 ** 21 + 5], 8, 16, True, 0)]
+
+
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_a_wait_that_runs_out_is_reported(case):
+    """The launch gives up, says so and leaves everything usable."""
+    job = _Product(*LONG[case])
+    want, status = job.run()
+    assert status == 0 and want.any()
+    with _wait_cycles(-1):
+        for _ in range(3):
+            _, status = job.run()
+            assert 41 <= status <= 49
+    again, status = job.run()
+    assert status == 0 and torch.equal(again, want)
