@@ -431,8 +431,8 @@ int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch, const void
                            int64_t w_expert_pitch, int contract_last, const int32_t* expert_offsets, int R, int E, int D0,
                            int D1, void* out_bf16, void* workspace, size_t workspace_bytes, int32_t* status,
                            b200moe_stream_t stream);
-/* How long a device-side wait of the products and of weight gradients launched from now on may take, in SM clocks, before the launch
- * gives up and reports it; 4000000000 (two seconds) until set.  Returns the value before. */
+/* How long products and weight gradients launched from now on may stand still, in SM clocks, before a device-side wait gives up and
+ * the launch reports it; 4000000000 (two seconds) until set.  Returns the value before. */
 int64_t b200moe_expert_wait_cycles(int64_t cycles);
 /* out[e] [M, N] = sum over the expert's rows r of a[r, :]^T b[r, :]; zero for an expert without rows. */
 size_t b200moe_expert_weight_grad_workspace_bytes(int R, int E, int M, int N);

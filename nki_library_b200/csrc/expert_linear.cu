@@ -128,17 +128,29 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t pa
       : "memory");
   return ok != 0;
 }
-// A wait's bound and where it is reported.
+// A wait's bound and where it is reported.  What is bounded is a standstill: an accumulator is waited for as long as its contraction
+// takes (2^24 slabs are 4 s), so the time starts again with every slab that the ring has taken on since.  These are finitely many.
 struct Bound {
-  volatile int* abort_flag;  // of the CTA
+  volatile int* abort_flag;     // of the CTA
+  const volatile int* started;  // slabs of the CTA's ring so far, modulo 2^32
   int32_t* status;
   int64_t cycles;
-  // Whether a wait that began at t0 is over without its barrier: its time is up or another warp of the CTA has given up.
-  __device__ __forceinline__ bool over(long long t0, int code) const {
-    if (*abort_flag) return true;
-    if (clock64() - t0 <= cycles) return false;
-    *abort_flag = 1;
-    atomicCAS(status, 0, code);
+};
+struct Clock {
+  const Bound& bound;
+  int seen;
+  long long t0;
+  // Whether the wait is over without its barrier: its time is up or another warp of the CTA has given up.
+  __device__ __forceinline__ bool over(int code) {
+    if (*bound.abort_flag) return true;
+    const int now = *bound.started;
+    if (now != seen) {
+      seen = now;
+      t0 = clock64();
+    }
+    if (clock64() - t0 <= bound.cycles) return false;
+    *bound.abort_flag = 1;
+    atomicCAS(bound.status, 0, code);
     return true;
   }
 };
@@ -148,16 +160,16 @@ template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Bound& bound, int code) {
   const auto done = [&] { return __all_sync(0xffffffffu, CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)); };
   if (done()) return true;
-  const long long t0 = clock64();
+  Clock clock{bound, *bound.started, clock64()};
   while (!done())
-    if (__any_sync(0xffffffffu, bound.over(t0, code))) return false;
+    if (__any_sync(0xffffffffu, clock.over(code))) return false;
   return true;
 }
 // One lane waits, the others do not.
 __device__ __forceinline__ bool lane_wait_cluster(uint64_t* bar, uint32_t parity, const Bound& bound, int code) {
-  const long long t0 = clock64();
+  Clock clock{bound, *bound.started, clock64()};
   while (!mbar_try_wait_cluster(bar, parity))
-    if (bound.over(t0, code)) return false;
+    if (clock.over(code)) return false;
   return true;
 }
 
@@ -295,6 +307,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
   uint64_t* queue_empty = queue_full + kQueue;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(queue_empty + kQueue);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  volatile int* started = abort_flag + 1;
   Sched& s = *reinterpret_cast<Sched*>(smem + C::kOffSched);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
@@ -317,7 +330,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
       mbar_init(&queue_full[a], 1);
       mbar_init(&queue_empty[a], 2 * (4 * kGroups + 2) + 1);  // every warp that walks the tiles
     }
-    *abort_flag = 0;
+    *abort_flag = *started = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -366,14 +379,14 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr;
   const int total = (WGRAD ? p.E * p.row_tiles * p.col_tiles : s.tiles[p.E]) * p.parts;
-  const Bound bound{abort_flag, p.status, p.wait_cycles};
+  const Bound bound{abort_flag, started, p.status, p.wait_cycles};
   Walk<!WGRAD> walk{p, s, queue_full, queue_empty, bound, unit, n_units, total, 0};
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer of the column operand
     const bool leader = elect_one();
     int stage = 0;
-    uint32_t phase = 0;
+    uint32_t phase = 0, taken_on = 0;
     bool ok = true;
     for (int tile = walk.next(); tile >= 0 && ok; tile = walk.next()) {
       const Tile t = decode_tile<WGRAD>(p, s, tile);
@@ -384,6 +397,7 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
         if (!warp_wait(&empty[stage], phase ^ 1u, bound, 41)) { ok = false; break; }
         uint8_t* dst = smem + stage * kStage;
         if (leader) {
+          *started = static_cast<int>(++taken_on);
           if (rank == 0) mbar_expect_tx(&full[stage], bytes);
           if constexpr (WGRAD) {
             tma2_load_2d(dst, &col_map, c, t.k0 + kb * 64, &full[stage]);

@@ -122,9 +122,11 @@ class _Product:
         gen = torch.Generator(device="cuda").manual_seed(K + N)
         self.E, self.R, self.K, self.N, self.weight_grad = len(counts), sum(counts) + behind, K, N, weight_grad
         self.offsets = torch.tensor([0] + counts).cumsum(0).int().cuda()
-        self.x = torch.randint(-2, 3, (self.R, K), device="cuda", generator=gen).bfloat16()
-        other = (self.R, N) if weight_grad else (self.E, K, N)
-        self.w = torch.randint(-2, 3, other, device="cuda", generator=gen).bfloat16()
+
+        def small(*shape):
+            return torch.randint(-2, 3, shape, device="cuda", generator=gen, dtype=torch.int8).bfloat16()
+
+        self.x, self.w = small(self.R, K), small(self.R, N) if weight_grad else small(self.E, K, N)
 
     def run(self):
         """(output, status)"""
@@ -151,6 +153,23 @@ class _Product:
 # tile per pair, tiles handed out, a weight gradient with ragged ends, parts of a contraction, parts of a weight gradient.
 LONG = [([3] * 40, 65536, 8, False, 0), ([8192], 65536, 8192, False, 3), ([70001] + [1] * 39, 8, 8, True, 0), ([5, 2], 2 ** 21, 16, False, 1),
         ([2 ** 21 + 5], 8, 16, True, 0)]
+
+
+# Contractions that take far longer than 400000 clocks (0.2 ms): one tile per pair; tiles handed out; a weight gradient; one whose
+# ragged ends are asked for behind tiles that have none.
+LONGER = [([3] * 40, 2 ** 19, 8, False, 0), ([8192], 2 ** 17, 2560, False, 3), ([2 ** 20 + 1] + [1] * 39, 8, 8, True, 0),
+          ([2 ** 18, 17], 2304, 2304, True, 0)]
+
+
+@pytest.mark.parametrize("case", range(len(LONGER)))
+def test_a_wait_lasts_as_long_as_the_contraction_moves_on(case):
+    """The limit is on a standstill: a contraction of 2^30 rows takes longer than any limit, and is right all the same."""
+    job = _Product(*LONGER[case])
+    want, status = job.run()
+    assert status == 0
+    with _wait_cycles(400000):
+        got, status = job.run()
+    assert status == 0 and torch.equal(got, want)
 
 
 @pytest.mark.parametrize("case", range(len(LONG)))
