@@ -424,7 +424,7 @@ int b200moe_unsort_rows_backward(const void* d_out, int64_t d_pitch, const void*
 /* Every expert's rows times its matrix, bf16 with fp32 accumulation.  weight: E matrices [D0, D1] with D1 contiguous
  * (pitches in elements).  contract_last 0: rows [R, D0] -> out [R, D1]; 1: rows [R, D1] -> out [R, D0].  Rows of no expert
  * come out zero.  D0 and D1 are multiples of 8; rows and matrices start on 16-byte boundaries.  status: device
- * int32[2], the first as for the grouped contractions (codes 41 to 49), the second scratch.  workspace: where few tiles
+ * int32[2], the first as for the grouped contractions (codes 41 to 49; out then holds NaN wherever it was not written), the second scratch.  workspace: where few tiles
  * have long contractions these are cut into parts, whose fp32 sums it holds (16-byte aligned; often 0 bytes). */
 size_t b200moe_expert_product_workspace_bytes(int contract_last, int R, int E, int D0, int D1);
 int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch, const void* weight_bf16, int64_t w_pitch,

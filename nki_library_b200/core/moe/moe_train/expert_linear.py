@@ -51,6 +51,9 @@ def expert_linear(rows: torch.Tensor, weight: torch.Tensor, expert_offsets: torc
 
     Differentiable in ``rows`` (zero in rows of no expert) and ``weight`` (zero for an expert without rows); gradients are
     bf16, summed in fp32 over an expert's rows only, whatever the other rows hold.
+
+    A product whose device-side wait runs out (it stands still for two seconds) ends and leaves NaN where it has written nothing;
+    with ``_check_status`` the call and its backward pass wait for their products and raise.
     """
     same_device(rows, weight, expert_offsets)
     if weight.dim() == 4:

@@ -12,13 +12,16 @@ from .sort_tokens import moe_sort_tokens, moe_unsort_tokens
 
 
 def moe_expert_mlp(rows: torch.Tensor, gate_up_proj_weight: torch.Tensor, down_proj_weight: torch.Tensor,
-                   expert_offsets: torch.Tensor, activation_function: ActFnType = ActFnType.SiLU) -> torch.Tensor:
+                   expert_offsets: torch.Tensor, activation_function: ActFnType = ActFnType.SiLU,
+                   _check_status: bool = False) -> torch.Tensor:
     """The experts' MLP on sorted rows: ``(act(gate) * up) @ down_proj_weight[e]`` with ``[gate, up] = rows @
     gate_up_proj_weight[e]``; ``rows [R, H]``, weights ``[E, H, 2, I]`` (or ``[E, H, 2 I]``) and ``[E, I, H]``, all bf16.
 
     The three operators in a row (:func:`expert_linear`, :func:`moe_glu`, :func:`expert_linear`), but what lives until the
     backward pass is the input rows and the 8-bit checkpoint of gate and up only: the activation in front of the down
     product is computed again from the checkpoint for the gradient of ``down_proj_weight``.
+
+    ``_check_status`` as in :func:`expert_linear`, of all products in both passes.
     """
     same_device(rows, gate_up_proj_weight, down_proj_weight, expert_offsets)
     A = _lib.kernel_assert
@@ -32,17 +35,17 @@ def moe_expert_mlp(rows: torch.Tensor, gate_up_proj_weight: torch.Tensor, down_p
       2 * down_proj_weight.shape[1] == gate_up_proj_weight.shape[2], "down_proj_weight must be bfloat16 [E, I, H_out]")
     A(down_proj_weight.shape[1] % 8 == 0 and down_proj_weight.shape[2] % 8 == 0 and
       0 < down_proj_weight.shape[2] <= MOST_COLUMNS, "both sizes of down_proj_weight's matrices must be multiples of 8, at most 2^27")
-    return native().mlp(rows, gate_up_proj_weight, down_proj_weight, expert_offsets, activation_function.value)
+    return native().mlp(rows, gate_up_proj_weight, down_proj_weight, expert_offsets, activation_function.value, _check_status)
 
 
 def moe_experts_train(hidden: torch.Tensor, affinities: torch.Tensor, expert_index: torch.Tensor,
                       gate_up_proj_weight: torch.Tensor, down_proj_weight: torch.Tensor,
-                      activation_function: ActFnType = ActFnType.SiLU) -> torch.Tensor:
+                      activation_function: ActFnType = ActFnType.SiLU, _check_status: bool = False) -> torch.Tensor:
     """The MoE layer behind its router, differentiable in ``hidden [T, H]``, ``affinities [T, K]`` and both weights:
     :func:`moe_sort_tokens` -> :func:`moe_expert_mlp` -> :func:`moe_unsort_tokens`.  ``expert_index [T, K]`` may hold ids
     outside ``[0, E)`` for dropped pairs; a token whose pairs are all dropped comes out zero.
     """
     same_device(hidden, affinities, expert_index, gate_up_proj_weight, down_proj_weight)
     rows, plan = moe_sort_tokens(hidden, expert_index, gate_up_proj_weight.shape[0])
-    out = moe_expert_mlp(rows, gate_up_proj_weight, down_proj_weight, plan.expert_offsets, activation_function)
+    out = moe_expert_mlp(rows, gate_up_proj_weight, down_proj_weight, plan.expert_offsets, activation_function, _check_status)
     return moe_unsort_tokens(out, affinities, plan)

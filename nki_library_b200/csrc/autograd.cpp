@@ -208,6 +208,12 @@ Stored stored(const Tensor& weight) {
   return {weight.clone(at::MemoryFormat::Contiguous), false};
 }
 
+// Waits for a product and raises if it has given up.
+void read_status(const Tensor& status) {
+  const int code = status[0].item<int>();
+  if (code != 0) throw EntryError("device-side wait expired in a product of the experts (status " + std::to_string(code) + ")");
+}
+
 // rows[r] @ weight[e], with `transpose` rows[r] @ weight[e].T
 Tensor product(const Tensor& rows, const Tensor& weight, const Tensor& offsets, bool transpose, bool check_status) {
   const On on(rows);
@@ -226,16 +232,12 @@ Tensor product(const Tensor& rows, const Tensor& weight, const Tensor& offsets, 
                                as_int(E), as_int(D0), as_int(D1), out.data_ptr(), address(ws), size, status.data_ptr<int>(),
                                on.stream),
         "b200moe_expert_product");
-  if (check_status) {
-    const int code = status[0].item<int>();
-    if (code != 0)
-      throw EntryError("device-side wait expired in expert_linear (status " + std::to_string(code) + ")");
-  }
+  if (check_status) read_status(status);
   return out;
 }
 
 // Gradient of product() in `weight`, laid out in memory as the weight is.
-Tensor weight_grad(const Tensor& rows, const Tensor& d_out, const Tensor& weight, const Tensor& offsets) {
+Tensor weight_grad(const Tensor& rows, const Tensor& d_out, const Tensor& weight, const Tensor& offsets, bool check_status) {
   const On on(weight);
   const bool turned = weight.stride(2) != 1 && weight.stride(1) == 1;
   const int64_t R = rows.size(0), E = weight.size(0), M = weight.size(turned ? 2 : 1), N = weight.size(turned ? 1 : 2);
@@ -252,6 +254,7 @@ Tensor weight_grad(const Tensor& rows, const Tensor& d_out, const Tensor& weight
                                      as_int(E), as_int(M), as_int(N), out.data_ptr(), address(ws), size, status.data_ptr<int>(),
                                      on.stream),
           "b200moe_expert_weight_grad");
+    if (check_status) read_status(status);
   }
   return turned ? out.transpose(1, 2) : out;
 }
@@ -259,15 +262,17 @@ Tensor weight_grad(const Tensor& rows, const Tensor& d_out, const Tensor& weight
 struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weight, const Tensor& offsets, bool check_status) {
     ctx->save_for_backward({weight.requires_grad() ? rows : Tensor(), weight, offsets});
+    ctx->saved_data["check"] = check_status;
     return product(rows, weight, offsets, false, check_status);
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) {
     refuse_transforms({d[0]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor d_out = tile_rows(d[0]);
+    const bool check = ctx->saved_data["check"].toBool();
     Tensor d_rows, d_weight;
-    if (ctx->needs_input_grad(0)) d_rows = product(d_out, saved[1], saved[2], true, false);
-    if (ctx->needs_input_grad(1)) d_weight = weight_grad(saved[0], d_out, saved[1], saved[2]);
+    if (ctx->needs_input_grad(0)) d_rows = product(d_out, saved[1], saved[2], true, check);
+    if (ctx->needs_input_grad(1)) d_weight = weight_grad(saved[0], d_out, saved[1], saved[2], check);
     return once({d_rows, d_weight, Tensor(), Tensor()});
   }
 };
@@ -321,11 +326,12 @@ struct Glu : torch::autograd::Function<Glu> {
 // ------------------------------------------------------------------ product, activation, product
 struct ExpertMLP : torch::autograd::Function<ExpertMLP> {
   static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& gate_up_weight, const Tensor& down_weight,
-                        const Tensor& offsets, int64_t act) {
-    auto [m, kept] = glu_forward(product(rows, gate_up_weight, offsets, false, false), act, true);
+                        const Tensor& offsets, int64_t act, bool check_status) {
+    auto [m, kept] = glu_forward(product(rows, gate_up_weight, offsets, false, check_status), act, true);
     ctx->save_for_backward({gate_up_weight.requires_grad() ? rows : Tensor(), gate_up_weight, down_weight, offsets, kept});
     ctx->saved_data["act"] = act;
-    return product(m, down_weight, offsets, false, false);
+    ctx->saved_data["check"] = check_status;
+    return product(m, down_weight, offsets, false, check_status);
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) {
     refuse_transforms({d[0]});
@@ -333,13 +339,14 @@ struct ExpertMLP : torch::autograd::Function<ExpertMLP> {
     const Tensor &rows = saved[0], &gate_up_weight = saved[1], &down_weight = saved[2], &offsets = saved[3];
     const bool want_rows = ctx->needs_input_grad(0), want_gate_up = ctx->needs_input_grad(1), want_down = ctx->needs_input_grad(2);
     const Tensor d_out = tile_rows(d[0]);
+    const bool check = ctx->saved_data["check"].toBool();
     Tensor d_m, d_rows, d_gate_up_weight, d_down;
-    if (want_rows || want_gate_up) d_m = product(d_out, down_weight, offsets, true, false);
+    if (want_rows || want_gate_up) d_m = product(d_out, down_weight, offsets, true, check);
     auto [d_gate_up, m] = glu_backward(d_m, saved[4], d_out.size(0), down_weight.size(1), ctx->saved_data["act"].toInt(), want_down);
-    if (want_down) d_down = weight_grad(m, d_out, down_weight, offsets);
-    if (want_rows) d_rows = product(d_gate_up, gate_up_weight, offsets, true, false);
-    if (want_gate_up) d_gate_up_weight = weight_grad(rows, d_gate_up, gate_up_weight, offsets);
-    return once({d_rows, d_gate_up_weight, d_down, Tensor(), Tensor()});
+    if (want_down) d_down = weight_grad(m, d_out, down_weight, offsets, check);
+    if (want_rows) d_rows = product(d_gate_up, gate_up_weight, offsets, true, check);
+    if (want_gate_up) d_gate_up_weight = weight_grad(rows, d_gate_up, gate_up_weight, offsets, check);
+    return once({d_rows, d_gate_up_weight, d_down, Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -372,14 +379,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, module) {
     return recorded({gate_up}) ? Glu::apply(gate_up, act) : std::get<0>(glu_forward(gate_up, act, false));
   });
   def("mlp", [](const Tensor& rows, const Tensor& gate_up_weight, const Tensor& down_weight, const Tensor& offsets,
-                       int64_t act) {
+                int64_t act, bool check_status) {
     refuse_transforms({rows, gate_up_weight, down_weight});
-    if (recorded({rows, gate_up_weight, down_weight})) return ExpertMLP::apply(rows, gate_up_weight, down_weight, offsets, act);
-    const Tensor m = std::get<0>(glu_forward(product(rows, gate_up_weight, offsets, false, false), act, false));
-    return product(m, down_weight, offsets, false, false);
+    if (recorded({rows, gate_up_weight, down_weight}))
+      return ExpertMLP::apply(rows, gate_up_weight, down_weight, offsets, act, check_status);
+    const Tensor m = std::get<0>(glu_forward(product(rows, gate_up_weight, offsets, false, check_status), act, false));
+    return product(m, down_weight, offsets, false, check_status);
   });
   def("product", &product);
-  def("weight_grad", &weight_grad);
+  def("weight_grad", [](const Tensor& rows, const Tensor& d_out, const Tensor& weight, const Tensor& offsets) {
+    return weight_grad(rows, d_out, weight, offsets, false);
+  });
   def("glu_forward", [](const Tensor& gate_up, int64_t act, bool keep) -> std::tuple<Tensor, Maybe> {
     auto [m, kept] = glu_forward(gate_up, act, keep);
     return {m, maybe(kept)};

@@ -27,8 +27,8 @@
 //          the 32 values a warp holds of a row are 64 contiguous bytes and go straight out.  Turning a chunk around in
 //          shared memory for longer stores costs the tensor pipe operand bandwidth, which the ring's copies and the MMAs
 //          use up (4 x 1024 rows, 4096 x 14336, weight grad: 361 us turned, 353 straight; 32 x 16 rows, 4096 x 4096: 248, 194).
-// Every wait is bounded; on expiry a code goes to `status`, no more work is issued and the kernel tears down, behind the copies and
-// MMAs that are under way.
+// Every wait is bounded; on expiry a code goes to `status`, no more work is issued, and the kernel tears down behind the copies and
+// MMAs that are under way and leaves NaN where it has written nothing.
 #include <cuda.h>
 
 #include <atomic>
@@ -636,6 +636,13 @@ expert_linear_kernel(const __grid_constant__ CUtensorMap col_map, const __grid_c
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+  }
+  if (*abort_flag) {
+    // Which tiles the pair still owed is not known here: all of the result (or of the parts' sums) becomes NaN, behind the pair's own
+    // stores, so that whatever is missing is one.  0x7fff7fff is NaN as fp32 and as two bf16.
+    uint4* to = p.parts > 1 ? reinterpret_cast<uint4*>(p.partial) : reinterpret_cast<uint4*>(p.out);
+    const int64_t values = p.parts * p.out_rows * p.cols, pieces = p.parts > 1 ? values / 4 : values / 8;
+    for (int64_t i = threadIdx.x; i < pieces; i += kThreads) to[i] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
   }
 }
 

@@ -180,7 +180,69 @@ def test_a_wait_that_runs_out_is_reported(case):
     assert status == 0 and want.any()
     with _wait_cycles(-1):
         for _ in range(3):
-            _, status = job.run()
+            got, status = job.run()
             assert 41 <= status <= 49
+            # nothing is taken for a result that is none
+            assert got.isnan().any() and (got.isnan() | (got == want)).all()
     again, status = job.run()
     assert status == 0 and torch.equal(again, want)
+
+
+def _long_layer():
+    import nki_library_b200 as m
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    E, R, H, I = 40, 120, 65536, 8
+    offsets = (torch.arange(E + 1, device="cuda") * (R // E)).int()
+    idx = (torch.arange(R, device="cuda") // (R // E)).int()[:, None]
+    rows = torch.randn((R, H), device="cuda", generator=gen).bfloat16().requires_grad_()
+    w1 = (torch.randn((E, H, 2 * I), device="cuda", generator=gen) * 0.01).bfloat16().requires_grad_()
+    w2 = torch.randn((E, I, H), device="cuda", generator=gen).bfloat16().requires_grad_()
+    ones = torch.ones((R, 1), device="cuda")
+    return {
+        "linear": (lambda check: m.expert_linear(rows, w1, offsets, _check_status=check), (rows, w1)),
+        "mlp": (lambda check: m.moe_expert_mlp(rows, w1, w2, offsets, _check_status=check), (rows, w1, w2)),
+        "layer": (lambda check: m.moe_experts_train(rows, ones, idx, w1, w2, _check_status=check), (rows, w1, w2)),
+    }
+
+
+@pytest.mark.parametrize("call", ["linear", "mlp", "layer"])
+def test_a_wait_that_runs_out_raises_or_leaves_nan(call):
+    """Asked for, in the forward pass and in the backward pass; else the results are NaN where nothing was written."""
+    fn, leaves = _long_layer()[call]
+    want = fn(False)
+    d = torch.ones_like(want)
+    for check in (False, True):
+        out = fn(check)
+        assert torch.equal(out, want)
+        grads = torch.autograd.grad(out, leaves, d, retain_graph=True)
+        if call == "linear":  # what has a long contraction here is the forward product; a layer's backward pass has one, too
+            continue
+        with _wait_cycles(-1):
+            if check:
+                with pytest.raises(AssertionError, match="wait expired"):
+                    torch.autograd.grad(out, leaves, d)
+            else:
+                got = torch.autograd.grad(out, leaves, d)
+                assert got[0].isnan().any() and got[1].isnan().any()
+                assert all(g.shape == w.shape for g, w in zip(got, grads))
+    with _wait_cycles(-1):
+        with pytest.raises(AssertionError, match="wait expired"):
+            fn(True)
+        with torch.no_grad(), pytest.raises(AssertionError, match="wait expired"):
+            fn(True)
+        assert fn(False).isnan().any()
+    assert torch.equal(fn(True), want)
+
+
+def test_a_gradient_whose_wait_runs_out_raises():
+    """Of the weights: 65537 rows of one expert."""
+    import nki_library_b200 as m
+    R, E = 65537 + 39, 40
+    offsets = torch.tensor([0] + [65537 + e for e in range(E)], dtype=torch.int32, device="cuda")
+    x = torch.ones((R, 8), dtype=torch.bfloat16, device="cuda")
+    w = torch.ones((E, 8, 8), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    out = m.expert_linear(x, w, offsets, _check_status=True)
+    with _wait_cycles(-1), pytest.raises(AssertionError, match="wait expired"):
+        torch.autograd.grad(out, w, torch.ones_like(out), retain_graph=True)
+    dw, = torch.autograd.grad(out, w, torch.ones_like(out))
+    assert (dw[0] == 65536).all() and (dw[1:] == 1).all()  # 65537 rounded to bf16

@@ -143,7 +143,7 @@ def _native_calls():
         "unsort": (lambda x, a: op.unsort(x, a, idx, off), [rows, torch.zeros(4, 2)]),
         "linear": (lambda x, w: op.linear(x, w, off, False), [rows, weight]),
         "glu": (lambda x: op.glu(x, 0), [rows]),
-        "mlp": (lambda x, w, v: op.mlp(x, w, v, off, 0), [rows, weight, down]),
+        "mlp": (lambda x, w, v: op.mlp(x, w, v, off, 0, False), [rows, weight, down]),
     }
 
 
