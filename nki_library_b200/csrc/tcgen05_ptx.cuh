@@ -271,20 +271,27 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+void* driver_entry(const char* name) {
+  void* ptr = nullptr;
+  cudaDriverEntryPointQueryResult found;
+  return cudaGetDriverEntryPoint(name, &ptr, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess ? ptr
+                                                                                                                            : nullptr;
+}
+
 EncodeTiledFn get_encode_fn() {
   static EncodeTiledFn fn = nullptr;
-  if (fn == nullptr) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  }
+  static CUresult (*get_current)(CUcontext*) = nullptr;
+  if (fn == nullptr) fn = reinterpret_cast<EncodeTiledFn>(driver_entry("cuTensorMapEncodeTiled"));
+  if (get_current == nullptr) get_current = reinterpret_cast<CUresult (*)(CUcontext*)>(driver_entry("cuCtxGetCurrent"));
   // The function wants a current context, which a host thread has only once it has set its device: not one that a framework
-  // has just started for a backward pass.
+  // has just started for a backward pass.  A thread that has one, be it a context of its own, keeps it.
   thread_local bool bound = false;
-  int dev = 0;
-  if (!bound && cudaGetDevice(&dev) == cudaSuccess) bound = cudaSetDevice(dev) == cudaSuccess;
+  if (!bound) {
+    CUcontext current = nullptr;
+    int dev = 0;
+    if (get_current != nullptr && get_current(&current) == CUDA_SUCCESS && current != nullptr) bound = true;
+    else if (cudaGetDevice(&dev) == cudaSuccess) bound = cudaSetDevice(dev) == cudaSuccess;
+  }
   return fn;
 }
 

@@ -246,3 +246,43 @@ def test_a_gradient_whose_wait_runs_out_raises():
         torch.autograd.grad(out, w, torch.ones_like(out), retain_graph=True)
     dw, = torch.autograd.grad(out, w, torch.ones_like(out))
     assert (dw[0] == 65536).all() and (dw[1:] == 1).all()  # 65537 rounded to bf16
+
+
+OWN_CONTEXT = """
+import ctypes, sys
+import numpy as np
+from nki_library_b200 import _lib
+cuda = ctypes.CDLL("libcuda.so.1")
+def ok(rc): assert rc == 0, rc
+context, now = ctypes.c_void_p(), ctypes.c_void_p()
+ok(cuda.cuInit(0))
+ok(cuda.cuCtxCreate_v2(ctypes.byref(context), 0, 0))
+def device(array):
+    p = ctypes.c_uint64()
+    ok(cuda.cuMemAlloc_v2(ctypes.byref(p), ctypes.c_size_t(array.nbytes)))
+    ok(cuda.cuMemcpyHtoD_v2(p, ctypes.c_void_p(array.ctypes.data), ctypes.c_size_t(array.nbytes)))
+    return p.value
+one = 0x3f80  # bf16 1
+x, w = (device(np.full(n, one, np.uint16)) for n in (64 * 128, 128 * 64))
+out, status = device(np.zeros(64 * 64, np.uint16)), device(np.full(2, -1, np.int32))
+offsets = device(np.array([0, 60], np.int32))
+lib = _lib.load_library()
+rc = lib.b200moe_expert_product(x, 128, w, 64, 128 * 64, 0, offsets, 64, 1, 128, 64, out, None, 0, status, None)
+assert rc == 0, lib.b200moe_last_error()
+ok(cuda.cuCtxGetCurrent(ctypes.byref(now)))
+assert now.value == context.value
+ok(cuda.cuCtxSynchronize())
+got = np.empty(64 * 64, np.uint16)
+ok(cuda.cuMemcpyDtoH_v2(ctypes.c_void_p(got.ctypes.data), ctypes.c_uint64(out), ctypes.c_size_t(got.nbytes)))
+assert (got.reshape(64, 64)[:60] == 0x4300).all() and not got.reshape(64, 64)[60:].any()  # 128
+"""
+
+
+def test_a_context_of_the_callers_own_stays_current():
+    """A C host with a context of the driver API: the first call of a thread makes a context current only where there is none."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", OWN_CONTEXT], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
