@@ -2,8 +2,12 @@
 
 import contextlib
 
+import math
+
 import pytest
 import torch
+
+import train_reference as ref
 
 pytestmark = pytest.mark.gpu
 
@@ -286,3 +290,88 @@ def test_a_context_of_the_callers_own_stays_current():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", OWN_CONTEXT], cwd=root, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+# ------------------------------------------------------------------ products of whole numbers
+MANY = [(7 * e) % 23 for e in range(300)]
+EXACT = [
+    # counts, K, N, rows behind the last expert
+    ([40001], 136, 8, 0), ([40001], 8, 136, 3), ([9000, 70, 0, 5003], 64, 72, 2), ([2 ** 20 + 17], 16, 8, 0),  # a weight gradient in parts
+    ([5, 0, 9], 4096, 72, 3), ([300], 8200, 520, 0), ([1], 2048, 8, 0), ([40, 700, 3], 64, 12000, 5),  # a product in parts
+    ([12000, 0, 3000, 1, 5199], 72, 14008, 40), ([12000, 0, 3000, 1, 5199], 1032, 13000, 0),  # tiles handed out
+    ([0, 15, 16, 17, 63, 64, 65, 0, 127, 128, 129, 255, 256, 257, 0], 328, 120, 300), ([700, 5, 1030], 1000, 776, 1), (MANY, 136, 304, 5),
+]
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("case", range(len(EXACT)))
+def test_products_of_whole_numbers_are_exact(case, transposed):
+    """Operands of -1 and 1: every partial sum is a whole number below 2^24, exact in fp32 in any order, so a result is the exact sum
+    rounded once.  A row or a step of the contraction that is missing or counted twice changes every sum by one, which shows in the
+    sums up to 256, whole numbers of bf16; the sums of n terms are of size sqrt(n)."""
+    import nki_library_b200 as m
+    counts, K, N, behind = EXACT[case]
+    gen = torch.Generator(device="cuda").manual_seed(case)
+
+    def signs(*shape):
+        return (torch.randint(0, 2, shape, device="cuda", generator=gen, dtype=torch.int8) * 2 - 1).bfloat16()
+
+    E, used = len(counts), sum(counts)
+    offsets = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    x, dy = signs(used + behind, K), signs(used + behind, N)
+    w = signs(E, N, K).transpose(1, 2) if transposed else signs(E, K, N)
+    x[used:], dy[used:] = math.nan, math.inf
+    x.requires_grad_(), w.requires_grad_()
+    y = m.expert_linear(x, w, offsets, _check_status=True)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    y, x, w = y.detach(), x.detach(), w.detach()
+    at = 0
+    for e, n in enumerate(counts):
+        part = slice(at, at + n)
+        at += n
+        xe, we, de = x[part].double(), w[e].double(), dy[part].double()
+        for got, want in ((y[part], xe @ we), (dx[part], de @ we.t()), (dw[e], xe.t() @ de)):
+            assert torch.equal(got, want.bfloat16()), e
+            if n * want.numel() > 0:
+                assert (want.abs() <= 256).any()
+    assert not y[at:].any() and not dx[at:].any()
+
+
+# ------------------------------------------------------------------ gradients of the activation far out
+FAR = [1e-30, 1e-3, 0.3, 1.0, 1.25, 2.0, 3.0, 4.0, 5.0, 6.0, 7.0, 8.0, 9.0, 10.0, 11.0, 12.0, 13.0, 14.0, 20.0, 40.0, 52.0, 60.0, 87.0, 90.0,
+       100.0, 300.0, 1e4, 1e10, 1e20, 1e30, 3e38, 3.38e38]
+
+
+@pytest.mark.parametrize("act", ["SiLU", "GELU", "GELU_Tanh_Approx", "Swish"])
+def test_gradient_of_far_gates(act):
+    """A row for each magnitude, so that its gates are kept at their size: both gradients of every column against the formula at the
+    kept values.
+
+    Bounds.  The kernel's exponentials have arguments of up to 127 powers of two, rounded up to five times to 2^-24: 127 * 5 * 2^-24 *
+    ln 2 = 2^-15.2, the approximations and products that follow add 2^-20 at most, GELU's fit 1.2e-6: 2^-15 of each of the slope's two
+    terms.  Where sigma is near one, 1 - sigma is off by 2^-22 and becomes zero from 24 powers of two on; times |g z'|, at most 35
+    there (the tanh form at 5): 2^-16.  What is flushed: sigma below 2^-126, times |g| <= 87.4 and |g z'| <= 232 (the tanh form at
+    -10.1): 2.8e-36 of the slope and 1.03e-36 of the activation."""
+    import nki_library_b200 as m
+    I = 32
+    base = torch.tensor([s * v for v in FAR for s in (-1, 1)], dtype=torch.float64)
+    gates = base[:, None] * (1 - torch.arange(I) / (2.0 * I))
+    gen = torch.Generator().manual_seed(2)
+    ups = torch.randint(0, 2, gates.shape, generator=gen) * 2 - 1
+    x = torch.cat([gates, ups], 1).bfloat16().cuda().requires_grad_()
+    d = ((torch.randint(0, 2, gates.shape, generator=gen) * 2 - 1) * 0.5).bfloat16().cuda()
+    grad, = torch.autograd.grad(m.moe_glu(x, m.ActFnType[act]), x, d)
+    _, g = ref.kept(x.detach()[:, :I])
+    _, u = ref.kept(x.detach()[:, I:])
+    assert torch.equal(u, x.detach()[:, I:].double()) and ((g.abs() / x.detach()[:, :I].double().abs() - 1).abs() <= 2.0 ** -4).all()
+    value, slope = ref.act_and_slope(g, act)
+    cdf = value / g  # sigma, or GELU's distribution function: the slope's first term
+    terms = cdf + (slope - cdf).abs()
+    want = torch.cat([d.double() * u * slope, d.double() * value], 1)
+    assert want.isfinite().all()
+    half = want.abs() * 2.0 ** -8 * (1 + 2.0 ** -8)
+    slack = torch.cat([terms * 2.0 ** -15 + (g > 0) * 2.0 ** -16 + 2.8e-36, value.abs() * 2.0 ** -15 + 1.03e-36], 1) * 0.5
+    off = (grad.double() - want).abs()
+    assert grad.isfinite().all()
+    worst = ((off - half - slack) / slack).amax(1)
+    assert (off <= half + slack).all(), [(float(base[i]), float(worst[i])) for i in (worst > 0).nonzero()[:, 0]]
