@@ -395,8 +395,8 @@ int b200moe_ep_return_rows(const void* y_pos_bf16, const int32_t* row_valid, con
                            b200moe_stream_t stream);
 
 /* ---- training pass of the experts -----------------------------------------------------------------
- * No counterpart in the reference's inference kernels.  Rows are sorted by expert without padding: expert e owns rows expert_offsets[e] to expert_offsets[e + 1] (int32 [E + 1], on the device) of R = T * K rows,
- * E <= 1024.  Limits: 2^31 - 1 pairs, 2^30 columns of sorted rows, 2^30 rows and matrices of 2^27 x 2^27 in a product, I up to 2^26.
+ * No counterpart in the reference's inference kernels.  Rows are sorted by expert without padding: expert e owns rows
+ * expert_offsets[e] to expert_offsets[e + 1] (int32 [E + 1], on the device) of R = T * K rows, E <= 1024.  Limits: 2^31 - 1 pairs, 2^30 columns of sorted rows, 2^30 rows and matrices of 2^27 x 2^27 in a product, I up to 2^26.
  *
  * sort_pairs: order of the pairs p = t * K + k of expert_index [T, K] (index_bytes 4 or 8) by (expert, p).  row_of_pair [T, K]
  * gets a pair's row, -1 where the id lies outside [0, E).  Up to 2048 pairs need no workspace. */

@@ -12,8 +12,9 @@ Public entry points mirror the reference (paths relative to its root):
 ``moe_block_tkg``      core/moe_block/moe_block_tkg.py:39
 =====================  ==========================================================
 
-and, without a counterpart there, the experts' training pass: ``moe_sort_plan``, ``moe_sort_tokens``,
-``moe_unsort_tokens``, ``expert_linear``, ``moe_glu``, ``moe_expert_mlp``, ``moe_experts_train``.
+and the experts' training pass in a form of its own (the reference's training kernels, experimental/moe/, are not mirrored):
+``moe_sort_plan``, ``moe_sort_tokens``, ``moe_unsort_tokens``, ``expert_linear``, ``moe_glu``, ``moe_expert_mlp``,
+``moe_experts_train``.
 
 All of them run hand-written sm_100a CUDA kernels through the C ABI in
 ``include/b200moe.h``; there is no CPU implementation in this package.

@@ -44,6 +44,10 @@ def moe_experts_train(hidden: torch.Tensor, affinities: torch.Tensor, expert_ind
     """The MoE layer behind its router, differentiable in ``hidden [T, H]``, ``affinities [T, K]`` and both weights:
     :func:`moe_sort_tokens` -> :func:`moe_expert_mlp` -> :func:`moe_unsort_tokens`.  ``expert_index [T, K]`` may hold ids
     outside ``[0, E)`` for dropped pairs; a token whose pairs are all dropped comes out zero.
+
+    Gradients come from an 8-bit checkpoint of gate and up (see :func:`moe_glu`), whose values are off by up to 2^-4 of themselves; that
+    of ``down_proj_weight`` is taken at the activation computed again from it, which is not bit for bit the one the forward pass
+    multiplied.
     """
     same_device(hidden, affinities, expert_index, gate_up_proj_weight, down_proj_weight)
     rows, plan = moe_sort_tokens(hidden, expert_index, gate_up_proj_weight.shape[0])

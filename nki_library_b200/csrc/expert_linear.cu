@@ -818,11 +818,16 @@ extern "C" int b200moe_expert_product(const void* rows_bf16, int64_t rows_pitch,
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Row tiles of an expert share its weight tiles in L2 as long as they run side by side.  A fixed walk drifts apart, since
   // tiles differ in width; handed out in order as pairs come free they stay together (32 experts of 7168 x 4096, 32768
-  // rows, skewed: 5.6 -> 2.8 GB from DRAM, 1533 -> 1356 us; its row gradient 3.6 -> 2.4 GB, 1440 -> 1342 us).  With one row
-  // tile per expert there is nothing to share, and with operands that L2 holds nothing to lose, while the counter's memset and
-  // the queue cost 4 to 9 us (64 experts of 2048 x 2048, 125 rows each: 109 us without, 118 with; 9216 rows on 6 experts of
-  // 64 x 13376: 64 and 73, of 4096 x 4096 211 and 215); so they do for the weight gradient's short contractions (4 x 1024
-  // rows, 4096 x 14336: 353 and 367 us).
+  // rows, skewed: 5.6 -> 2.8 GB from DRAM, 1533 -> 1356 us; its row gradient 3.6 -> 2.4 GB, 1440 -> 1342 us).  The drift is a few
+  // tiles, so it costs nothing until the operands are many times L2, while the counter's memset and the queue cost 4 us and more.
+  // Fixed / handed out by the operands' size, two or more row tiles per expert: 71 MB (16000 rows, 256 x 32768) 422 / 440 us, 95 MB
+  // (64000 rows) 1352 / 1439, 160 MB (8192 rows, 2048 x 4096) 97 / 100, 320 MB (4096 x 4096) 190 / 195 and its row gradient 209 / 217,
+  // 576 MB (4096 x 8192) 415 / 418, 605 MB (24000 rows, 2048 x 4096) 372 / 381, 737 MB (skewed) 780 / 776, 960 MB (4096 x 14336)
+  // 758 / 753, 1.2 GB (skewed) 1569 / 1549, 2.0 GB (24000 rows, 7168 x 4096) 1339 / 1292 and 1294 / 1246: half a gigabyte is where loss
+  // turns into gain.  One row tile per expert has nothing to share.  The weight gradient's short contractions lose everywhere
+  // (4 x 1024 rows, 4096 x 14336: 353 and 367 us).
+  // The queue holds two tiles, four where contractions are too short to hide a ticket's way (256 x 32768 above: 462 us with two,
+  // 440 with four; from 1024 on the two are within 2 % of each other, either way).
   const int64_t bytes = 2 * (static_cast<int64_t>(E) * D0 * D1 + static_cast<int64_t>(R) * k);
   if (R >= 512 * static_cast<int64_t>(E) && bytes >= (int64_t{1} << 29) && most_tiles >= 4 * (sm_count() / 2)) {
     p.taken = status + 1;

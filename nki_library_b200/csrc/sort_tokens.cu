@@ -781,8 +781,9 @@ extern "C" int b200moe_sort_tokens(const void* hidden, int dtype, int64_t pitch,
   if (rc != B200MOE_OK) return rc;
   rc = check_sort(expert_index, index_bytes, T, K, E, expert_offsets, row_of_pair);
   if (rc != B200MOE_OK) return rc;
-  // One launch instead of two where a CTA per token does not repeat the order too often (16 tokens of 4096, 128 experts, top-8: 7.0 us
-  // instead of 4.8 + 3.8, and 16.6 instead of 19.3 of host time)
+  // One launch instead of two where a CTA per token does not repeat the order too often.  One / two launches, back to back, tokens of
+  // 4096, 128 experts, top-8: 16 tokens 5.1 / 7.4 us, 64 5.4 / 7.4, 128 6.9 / 7.4, 160 9.5 / 7.9, 256 10.1 / 9.4 (8 experts: 128 5.7 /
+  // 7.4, 256 7.4 / 7.8; 1024 experts: 128 7.3 / 8.4, 160 10.8 / 9.1).
   if (static_cast<int64_t>(T) * K <= kChunk && T <= 128) {
     widen_copy(dtype, H, pitch, hidden, rows);
     const SortArgs s{expert_index, index_bytes == 8, static_cast<int64_t>(T) * K, E};
@@ -816,6 +817,9 @@ extern "C" int b200moe_unsort_rows(const void* rows, int dtype, int64_t pitch, i
     using T_ = decltype(element);
     constexpr bool W = decltype(whole)::value;
     const Layout l = row_layout(T, H, kPer<T_>, 128, true);
+    // Rows in flight, four / eight: 32768 tokens of 4096 bf16, top-8 356 / 347 us, of 2048 185 / 180 (fp32 687 / 690), where several
+    // tokens share a CTA 111 / 118 (65536 of 512); cut rows, whose reads take three registers more each, of 2045 251 / 368; with top-2
+    // (16384 of 4096) 76 / 85.
     const auto kernel = l.block.y > 1 ? (K > 4 ? unsort_rows_kernel<T_, W, true, W ? 8 : 4> : unsort_rows_kernel<T_, W, true, 4>)
                                       : (K > 4 ? unsort_rows_kernel<T_, W, false, W ? 8 : 4> : unsort_rows_kernel<T_, W, false, 4>);
     B200MOE_CUDA_OK(launch_overlapped(kernel, l.grid, l.block, 0, static_cast<cudaStream_t>(stream), a,
@@ -847,6 +851,9 @@ extern "C" int b200moe_unsort_rows_backward(const void* d_out, int64_t d_pitch, 
                    [&](auto element, auto whole) -> int {
     using T_ = decltype(element);
     constexpr bool W = decltype(whole)::value;
+    // Threads of a CTA, 128 / 256: 32768 tokens, top-8, bf16 of 2048 344 / 455 us, 4096 683 / 733, 8192 1373 / 1384, 16384 (16384 tokens,
+    // top-4) 742 / 726; fp32 of 2048 684 / 737, 4096 1373 / 1363, 8192 2772 / 2718.  Few tokens leave SMs idle, and the wider CTA is
+    // through sooner where they do: 64 of 4096 fp32 10.4 / 9.3, bf16 8.6 / 8.4 (300 11.0 / 11.4, 600 12.3 / 14.7).
     const int threads = T >= 8 * sm_count() && H <= 128 * 8 * kPer<T_> ? 128 : 256;
     const Layout l = row_layout(T, H, kPer<T_>, threads, false);
     const bool few_tokens = T <= 2 * sm_count();  // all of them at once in the form of eight rows
